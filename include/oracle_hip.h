@@ -181,6 +181,61 @@ int64_t orc_decode_stream_bytes(orc_engine* e, int which);
  * No counterpart in the reference (measurement only). */
 int orc_decode_weight_stats(orc_engine* e, int64_t* out6);
 
+/* ---- operators: prompts of different lengths in one pass, and a paged KV cache (no counterpart in the reference, whose batches
+ * are left-padded and whose cache is one tensor per layer: llava_arch.py:192-201, llava_llama.py:54-112) --------------------
+ * dtype: 0 = bf16, 1 = fp16; head_dim 64 or 128; query head h reads K/V head h / (n_heads / n_kv_heads). Strides are in
+ * elements, multiples of 8 (the innermost dimension is contiguous), and every tensor starts on 16 bytes. Asynchronous on
+ * `stream`, no allocation, no host synchronisation: every call can be captured into a graph.
+ *
+ * orc_attn_plan (host only): the query tiles of n sequences that lie one behind the other, lens_host[i] >= 0 tokens each, `bm`
+ * query rows per tile, longest key range first; four ints a tile (first token of the sequence, its length, first query row of the tile in it,
+ * 0) to out_host. Returns the number of tiles (out_host may be NULL to count them), -1 on error.
+ * orc_attn_tile (host only): the tile height to plan for: 128, or 256 where the prompts are long enough to fill the GPU with those.
+ * orc_attention_packed: causal attention inside every sequence, token t of a sequence over its tokens 0..t.
+ * q (total, n_heads, head_dim), k / v (total, n_kv_heads, head_dim), out like q; strides8 = {q token, q head, k token, k head,
+ * v token, v head, out token, out head}; work = the plan on the device. Rows of `out` that no sequence covers are left as they are. */
+int orc_attn_plan(const int32_t* lens_host, int n, int bm, int32_t* out_host, int capacity);
+int orc_attn_tile(const int32_t* lens_host, int n, int n_heads);
+int orc_attention_packed(const void* q, const void* k, const void* v, void* out, const int64_t* strides8, const int32_t* work, int n_work,
+                         int bm, int total, int n_heads, int n_kv_heads, int head_dim, int dtype, float scale, void* stream);
+
+/* A paged KV cache. The caller owns every array (device): kv [n_layers][2 (K, V)][n_pages][n_kv_heads][page_size][head_dim];
+ * table [max_rows][max_row_pages], page of every page_size tokens of a row, -1 behind its last page; lens [max_rows] tokens held; refs [n_pages]
+ * rows that hold a page (0 = free); status [1], sticky ORC_KV_* bits; work [ORC_KV_WORK_INTS(...)] scratch.
+ * A page that more than one row holds is full, so it is never written again. The calls on one cache are ordered by the caller (one stream, or events).
+ * A call whose lists are wrong or that finds too few free pages sets its bit in `status` and changes nothing else. Lists are
+ * device arrays; n <= 1024 rows, 2^20 tokens, a call. Fresh pages are the lowest free ones, taken in the order of the list. page_size 16, 32, 64 or 128. */
+typedef struct orc_kv_pages {
+  void* kv;
+  int32_t *table, *lens, *refs, *status, *work;
+  int32_t n_layers, n_pages, n_kv_heads, page_size, head_dim, max_rows, max_row_pages, dtype;
+} orc_kv_pages;
+#define ORC_KV_WORK_INTS(n_pages) (8 + 4 * (n_pages))
+enum { ORC_KV_BAD_ROW = 1, ORC_KV_ROW_TWICE = 2, ORC_KV_BAD_COUNT = 4, ORC_KV_ROW_FULL = 8, ORC_KV_POOL_FULL = 16, ORC_KV_NOT_EMPTY = 32,
+       ORC_KV_BAD_PAGE = 64, ORC_KV_NOT_SHARED = 128 };
+/* counts[i] more tokens (NULL: one) for row rows[i]; slots[0..total): place (page * page_size + offset) of every new token, the rows' tokens
+ * one behind the other in list order, -1 behind the last and everywhere when the call fails. */
+int orc_kv_reserve(const orc_kv_pages* c, const int32_t* rows, const int32_t* counts, int n, int32_t* slots, int total, void* stream);
+/* K / V of `total` tokens (token and head strides in elements) into their slots of one layer; a slot outside the pool is skipped. */
+int orc_kv_append(const orc_kv_pages* c, int layer, const int32_t* slots, int total, const void* k, const void* v, const int64_t* strides4,
+                  void* stream);
+/* Row dst[i] (empty) becomes row src[i], or its first n_tokens tokens (n_tokens < 0: all). share != 0: full pages are shared and the part page
+ * is copied; share == 0: every page is copied. A src row may be named more than once. */
+int orc_kv_fork(const orc_kv_pages* c, const int32_t* src, const int32_t* dst, int n, int n_tokens, int share, void* stream);
+/* Rows give their pages back (an empty row: nothing). */
+int orc_kv_free(const orc_kv_pages* c, const int32_t* rows, int n, void* stream);
+/* Held pages to the front. into == NULL: in place, pages behind the last to keep move into the holes, lowest first. Otherwise into another
+ * cache of the same geometry (n_pages may differ), whose rows become copies of these; page order is kept and `c` stays as it is. */
+int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, void* stream);
+/* One token of attention per query over the cache: query i (q [n][n_heads][head_dim], strides4 = {q token, q head, out token, out head}) reads
+ * the first limits[i] tokens (NULL: all lens[rows[i]]) of row rows[i]. The first prefix_tokens (a multiple of page_size) are held
+ * on the same pages by every named row and are read once for all of them, through rows[0]; rows that do not share them set
+ * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros. Tokens on a page outside the pool are not attended.
+ * ws: orc_kv_attend_ws bytes of scratch, 16-byte aligned. */
+int64_t orc_kv_attend_ws(const orc_kv_pages* c, int n, int n_heads, int prefix_tokens);
+int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, void* out, const int64_t* strides4, const int32_t* rows, const int32_t* limits,
+                  int n, int n_heads, int prefix_tokens, float scale, void* ws, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

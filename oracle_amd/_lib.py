@@ -22,6 +22,11 @@ class OrcConfig(C.Structure):
     ]
 
 
+class OrcKvPages(C.Structure):
+    _fields_ = [(x, C.c_void_p) for x in ('kv', 'table', 'lens', 'refs', 'status', 'work')] + \
+               [(x, C.c_int32) for x in ('n_layers', 'n_pages', 'n_kv_heads', 'page_size', 'head_dim', 'max_rows', 'max_row_pages', 'dtype')]
+
+
 # every symbol include/oracle_hip.h declares: (restype, argtypes)
 _P, _I, _F, _L = C.c_void_p, C.c_int, C.c_float, C.c_int64
 SYMBOLS = {
@@ -62,6 +67,16 @@ SYMBOLS = {
     'orc_kv_bytes_per_key': (_L, [_P]),
     'orc_decode_stream_bytes': (_L, [_P, _I]),
     'orc_decode_weight_stats': (_I, [_P, C.POINTER(_L)]),
+    'orc_attn_plan': (_I, [_P, _I, _I, _P, _I]),
+    'orc_attn_tile': (_I, [_P, _I, _I]),
+    'orc_attention_packed': (_I, [_P, _P, _P, _P, C.POINTER(_L), _P, _I, _I, _I, _I, _I, _I, _I, _F, _P]),
+    'orc_kv_reserve': (_I, [C.POINTER(OrcKvPages), _P, _P, _I, _P, _I, _P]),
+    'orc_kv_append': (_I, [C.POINTER(OrcKvPages), _I, _P, _I, _P, _P, C.POINTER(_L), _P]),
+    'orc_kv_fork': (_I, [C.POINTER(OrcKvPages), _P, _P, _I, _I, _I, _P]),
+    'orc_kv_free': (_I, [C.POINTER(OrcKvPages), _P, _I, _P]),
+    'orc_kv_compact': (_I, [C.POINTER(OrcKvPages), C.POINTER(OrcKvPages), _P]),
+    'orc_kv_attend_ws': (_L, [C.POINTER(OrcKvPages), _I, _I, _I]),
+    'orc_kv_attend': (_I, [C.POINTER(OrcKvPages), _I, _P, _P, C.POINTER(_L), _P, _P, _I, _I, _I, _F, _P, _P]),
 }
 
 

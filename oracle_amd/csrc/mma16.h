@@ -1,0 +1,38 @@
+// The two 16-bit element types of the attention operators (attn_packed.hip, attn_paged.hip) and their matrix instructions.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(1))) const void glb_void_t;
+
+template <typename T> struct Mma;
+template <> struct Mma<__bf16> {
+  typedef bf16x8 v8;
+  typedef __attribute__((ext_vector_type(2))) __bf16 v2;
+  static __device__ __forceinline__ f32x16 m32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 m16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<_Float16> {
+  typedef f16x8 v8;
+  typedef __attribute__((ext_vector_type(2))) _Float16 v2;
+  static __device__ __forceinline__ f32x16 m32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 m16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+// two floats rounded to nearest even, packed
+template <typename T> __device__ __forceinline__ uint32_t cvt2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, typename Mma<T>::v2));
+}
+// 4 rows x 16 columns of 16-bit values, transposed by a group of 16 lanes: lane i passes the address of 8 bytes (row i / 4, columns
+// 4 (i % 4) ...) and gets column i, rows 0..3
+template <typename T> __device__ __forceinline__ u32x2 lds_tr16(const char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p));
+}
+template <typename T> __device__ __forceinline__ typename Mma<T>::v8 join8(u32x2 a, u32x2 b) {
+  return __builtin_bit_cast(typename Mma<T>::v8, (u32x4){a[0], a[1], b[0], b[1]});
+}

@@ -1,0 +1,286 @@
+"""Prompts of different lengths in one pass, and a paged KV cache: attention over packed prompts (`packed_attention`), and `KvPages` --
+pages taken and filled (`reserve`, `append`), shared and copied (`fork`, `copy`), given back (`free`), moved together (`compact`), and
+decode attention that reads a prefix shared by the whole batch once (`attend`). The C entry points are orc_attention_packed and
+orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .engine import _ptr
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ERRORS = ((1, 'a row outside the table'), (2, 'a row named twice (or a fork onto one of its sources)'), (4, 'a bad token count'),
+           (8, 'a row longer than the table is wide'), (16, 'too few free pages'), (32, 'a fork onto a row that holds tokens'),
+           (64, 'a page outside the pool'), (128, 'rows that do not share the prefix they were attended with'))
+
+
+def _on(t):
+    """(stream of t's GPU, context that makes that GPU the current one)"""
+    i = t.device.index
+    return C.c_void_p(torch.cuda.current_stream(i).cuda_stream), torch.cuda.device(i)
+
+
+def _chk(t, name, dim, dtype=None, device=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f'{name} must be a CUDA tensor')
+    if t.dim() != dim:
+        raise ValueError(f'{name} must have {dim} dimensions, got {tuple(t.shape)}')
+    if dtype is None:
+        if t.dtype not in _DTYPES:
+            raise ValueError(f'{name} must be bfloat16 or float16, got {t.dtype}')
+    elif t.dtype != dtype:
+        raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
+    if device is not None and t.device != device:
+        raise ValueError(f'{name} is on {t.device}, not on {device}')
+
+
+def _strides(t, name):
+    """(token stride, head stride) of (tokens, heads, head_dim)"""
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f'{name}: the last dimension must be contiguous')
+    ts, hs = (t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+    if ts < 0 or hs < 0 or ts % 8 or hs % 8 or t.data_ptr() % 16:
+        raise ValueError(f'{name}: token and head strides must be multiples of 8 elements and the tensor must start on 16 bytes, '
+                         f'got strides {tuple(t.stride())} at {t.data_ptr() % 16} bytes past 16')
+    return ts, hs
+
+
+def _overlaps_itself(t):
+    """whether two of t's elements may share memory (an output must not be an expanded view)"""
+    need = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda x: x[1]):
+        if size > 1:
+            if stride < need:
+                return True
+            need = stride * (size - 1) + need
+    return False
+
+
+def _ints(t, name, device, n=None):
+    _chk(t, name, 1, torch.int32, device)
+    if not t.is_contiguous():
+        raise ValueError(f'{name} must be contiguous')
+    if n is not None and t.numel() != n:
+        raise ValueError(f'{name} must hold {n} values, got {t.numel()}')
+    return _ptr(t)
+
+
+def _out(out, like, name='out'):
+    if out is None:
+        return None
+    _chk(out, name, 3, like.dtype, like.device)
+    if out.shape != like.shape:
+        raise ValueError(f'{name} must have the shape {tuple(like.shape)}, got {tuple(out.shape)}')
+    if _overlaps_itself(out):
+        raise ValueError(f'{name} must not be an expanded view')
+    return out
+
+
+class PackedPlan:
+    """The query tiles of prompts that lie one behind the other, `lens` tokens each (0 allowed), on `device`: made once for a batch
+    and used for every layer. It holds for any number of heads."""
+
+    def __init__(self, lens, device='cuda', n_heads=32):
+        self.lens = [int(x) for x in lens]
+        n = len(self.lens)
+        if any(x < 0 or x > 0x7fffffff for x in self.lens) or sum(self.lens) > 0x7fffffff:
+            raise ValueError('lengths must not be negative, nor add up to more than 2^31 - 1')
+        self.total = sum(self.lens)
+        lib = _lib.lib()
+        arr = (C.c_int32 * max(n, 1))(*self.lens)
+        self.tile = lib.orc_attn_tile(arr, n, int(n_heads))
+        self.n_work = lib.orc_attn_plan(arr, n, self.tile, None, 0)
+        if self.n_work < 0:
+            _lib.check(self.n_work, 'orc_attn_plan')
+        work = torch.empty(max(self.n_work, 1), 4, dtype=torch.int32)
+        if lib.orc_attn_plan(arr, n, self.tile, _ptr(work), self.n_work) < 0:
+            _lib.check(-1, 'orc_attn_plan')
+        self.work = work.to(device)
+
+
+def packed_attention(q, k, v, plan, scale=None, out=None):
+    """Causal attention inside every prompt of `plan`: q (T, Hq, hd), k / v (T, Hkv, hd) with T >= plan.total, hd 64 or 128, Hq a multiple of
+    Hkv; slices of a fused projection are taken as they are. scale defaults to hd ** -0.5. Rows of `out` behind the last prompt are left
+    as they are (zero in a tensor made here)."""
+    _chk(q, 'q', 3)
+    _chk(k, 'k', 3, q.dtype, q.device)
+    _chk(v, 'v', 3, q.dtype, q.device)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f'q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together')
+    hq, hkv, hd = q.shape[1], k.shape[1], q.shape[2]
+    if hd not in (64, 128):
+        raise ValueError(f'head_dim must be 64 or 128, got {hd}')
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError(f'{hq} query heads are not a multiple of {hkv} K/V heads')
+    if plan.total > q.shape[0]:
+        raise ValueError(f'the plan covers {plan.total} tokens, q has {q.shape[0]}')
+    if plan.work.device != q.device:
+        raise ValueError(f'the plan is on {plan.work.device}, not on {q.device}')
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f'scale must be positive and finite, got {scale}')
+    out = _out(out, q)
+    if out is None:
+        out = (torch.empty if plan.total == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    st = (C.c_int64 * 8)(*_strides(q, 'q'), *_strides(k, 'k'), *_strides(v, 'v'), *_strides(out, 'out'))
+    stream, dev = _on(q)
+    with dev:
+        _lib.check(_lib.lib().orc_attention_packed(_ptr(q), _ptr(k), _ptr(v), _ptr(out), st, _ptr(plan.work), plan.n_work, plan.tile, plan.total,
+                                                   hq, hkv, hd, _DTYPES[q.dtype], scale, stream), 'orc_attention_packed')
+    return out
+
+
+class KvPages:
+    """A paged KV cache. kv (n_layers, 2, n_pages, n_kv_heads, page_size, head_dim) holds the tokens; table (max_rows, max_row_pages) the
+    pages of every row (-1: none), lens (max_rows,) its tokens, refs (n_pages,) how many rows hold a page -- all on the GPU, so no call waits for it
+    and all of them can be captured into a graph. Lists of rows and counts are int32 tensors there. A call whose lists are wrong, or that
+    finds too few free pages, changes nothing and leaves a note that `check()` raises. The caller orders the calls on one cache (one
+    stream, or events). A page that several rows hold is full and is not written again."""
+
+    def __init__(self, n_layers, n_pages, n_kv_heads, head_dim, page_size=64, max_rows=64, max_row_pages=64, dtype=torch.bfloat16, device='cuda'):
+        if min(n_layers, n_pages, n_kv_heads, max_rows, max_row_pages) < 1:
+            raise ValueError('every size of the cache must be at least 1')
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError(f'page_size must be 16, 32, 64 or 128, got {page_size}')
+        if head_dim not in (64, 128):
+            raise ValueError(f'head_dim must be 64 or 128, got {head_dim}')
+        if dtype not in _DTYPES:
+            raise ValueError(f'dtype must be bfloat16 or float16, got {dtype}')
+        i32 = dict(dtype=torch.int32, device=device)
+        self._adopt(torch.zeros(n_layers, 2, n_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device),
+                    torch.full((max_rows, max_row_pages), -1, **i32), torch.zeros(max_rows, **i32), torch.zeros(n_pages, **i32))
+
+    @classmethod
+    def wrap(cls, kv, table, lens, refs):
+        """A cache over tensors that exist already, in the layout of the class; they are used, not copied."""
+        self = cls.__new__(cls)
+        self._adopt(kv, table, lens, refs)
+        return self
+
+    def _adopt(self, kv, table, lens, refs):
+        _chk(kv, 'kv', 6)
+        for t, name, dim in ((table, 'table', 2), (lens, 'lens', 1), (refs, 'refs', 1)):
+            _chk(t, name, dim, torch.int32, kv.device)
+        if not all(t.is_contiguous() for t in (kv, table, lens, refs)) or kv.data_ptr() % 16:
+            raise ValueError('kv, table, lens and refs must be contiguous, and kv must start on 16 bytes')
+        layers, two, n_pages, hkv, page, hd = kv.shape
+        if two != 2 or page not in (16, 32, 64, 128) or hd not in (64, 128) or min(layers, n_pages, hkv) < 1:
+            raise ValueError(f'kv must be (n_layers, 2, n_pages, n_kv_heads, 16 | 32 | 64 | 128, 64 | 128), got {tuple(kv.shape)}')
+        if lens.numel() != table.shape[0] or refs.numel() != n_pages or not 1 <= table.shape[0] <= 65536 or not 1 <= table.shape[1] <= 1 << 20:
+            raise ValueError(f'table {tuple(table.shape)}, lens {tuple(lens.shape)} and refs {tuple(refs.shape)} do not belong to {n_pages} pages')
+        if n_pages * page > 0x7fffffff:
+            raise ValueError('the pool holds more than 2^31 - 1 tokens')
+        self.kv, self.table, self.lens, self.refs = kv, table, lens, refs
+        self.device, self.page_size, self.n_layers = kv.device, page, layers
+        self.status = torch.zeros(1, dtype=torch.int32, device=kv.device)
+        self._work = torch.zeros(8 + 4 * n_pages, dtype=torch.int32, device=kv.device)
+        self._c = _lib.OrcKvPages(*[t.data_ptr() for t in (kv, table, lens, refs, self.status, self._work)], layers, n_pages, hkv, page, hd,
+                                  table.shape[0], table.shape[1], _DTYPES[kv.dtype])
+
+    def _call(self, name, *args):
+        stream, dev = _on(self.kv)
+        with dev:
+            _lib.check(getattr(_lib.lib(), name)(C.byref(self._c), *args, stream), name)
+
+    def _rows(self, rows, name='rows', n=None):
+        p = _ints(rows, name, self.device, n)
+        if rows.numel() > 1024:
+            raise ValueError(f'{name}: at most 1024 rows a call, got {rows.numel()}')
+        return p
+
+    def check(self):
+        """Waits for the GPU and raises if a call since the last check was refused there."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise _lib.OracleHipError('KvPages: ' + '; '.join(text for bit, text in _ERRORS if bits & bit))
+
+    def reserve(self, rows, counts=None, total=None):
+        """Room for counts[i] more tokens (None: one) of every row: takes the lowest free pages and returns the new tokens' places (int32, `total` of
+        them, the rows' tokens one behind the other, -1 behind the last) for `append`. total: the sum of counts, which the host has to know; it
+        may be larger."""
+        r = self._rows(rows)
+        n = rows.numel()
+        c = None if counts is None else _ints(counts, 'counts', self.device, n)
+        if total is None:
+            if counts is not None:
+                raise ValueError('total is needed with counts')
+            total = n
+        if not 0 <= total <= 1 << 20:
+            raise ValueError(f'total must be 0..2^20, got {total}')
+        slots = torch.empty(total, dtype=torch.int32, device=self.device)
+        self._call('orc_kv_reserve', r, c, n, _ptr(slots), int(total))
+        return slots
+
+    def append(self, layer, slots, k, v):
+        """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`; a place of -1 is skipped."""
+        _chk(k, 'k', 3, self.kv.dtype, self.device)
+        _chk(v, 'v', 3, self.kv.dtype, self.device)
+        want = (slots.numel(), self.kv.shape[3], self.kv.shape[5])
+        if tuple(k.shape) != want or tuple(v.shape) != want:
+            raise ValueError(f'k {tuple(k.shape)} and v {tuple(v.shape)} must be {want}')
+        self._layer(layer)
+        st = (C.c_int64 * 4)(*_strides(k, 'k'), *_strides(v, 'v'))
+        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), slots.numel(), _ptr(k), _ptr(v), st)
+
+    def _layer(self, layer):
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f'layer {layer} outside 0..{self.n_layers - 1}')
+
+    def _fork(self, src, dst, n_tokens, share):
+        n_tokens = -1 if n_tokens is None else int(n_tokens)
+        if n_tokens < -1 or n_tokens > 0x7fffffff:
+            raise ValueError('n_tokens must not be negative')
+        self._call('orc_kv_fork', self._rows(src, 'src'), self._rows(dst, 'dst', src.numel()), src.numel(), n_tokens, share)
+
+    def fork(self, src, dst, n_tokens=None):
+        """The empty rows dst[i] become rows src[i] (their first n_tokens tokens): full pages are shared, the part page is copied. A row can be
+        forked to many; no src row may be among dst."""
+        self._fork(src, dst, n_tokens, 1)
+
+    def copy(self, src, dst, n_tokens=None):
+        """As `fork`, with pages of their own for every token."""
+        self._fork(src, dst, n_tokens, 0)
+
+    def free(self, rows):
+        """The rows give their pages back and hold no tokens."""
+        self._call('orc_kv_free', self._rows(rows), rows.numel())
+
+    def compact(self, into=None):
+        """Held pages to the front of the pool: in place, the pages that stick out move into the holes. into: another cache of the same geometry
+        (n_pages may differ), which becomes a copy of this one without the holes; this one stays as it is."""
+        if into is not None and into.device != self.device:
+            raise ValueError(f'into is on {into.device}, not on {self.device}')
+        self._call('orc_kv_compact', None if into is None else C.byref(into._c))
+
+    def attend(self, layer, q, rows, prefix_tokens=0, limits=None, scale=None, out=None):
+        """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
+        n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
+        once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
+        gives zeros."""
+        _chk(q, 'q', 3, self.kv.dtype, self.device)
+        n, hq, hd = q.shape
+        if hd != self.kv.shape[5]:
+            raise ValueError(f'head_dim of q is {hd}, of the cache {self.kv.shape[5]}')
+        hkv = self.kv.shape[3]
+        if hq < 1 or hq % hkv:
+            raise ValueError(f'{hq} query heads are not a multiple of {hkv} K/V heads')
+        self._layer(layer)
+        if prefix_tokens < 0 or prefix_tokens % self.page_size or prefix_tokens > self.table.shape[1] * self.page_size:
+            raise ValueError(f'prefix_tokens must be a multiple of page_size {self.page_size} inside a row, got {prefix_tokens}')
+        r = self._rows(rows, n=n)
+        lim = None if limits is None else _ints(limits, 'limits', self.device, n)
+        scale = hd ** -0.5 if scale is None else float(scale)
+        if not 0.0 < scale < 1e30:
+            raise ValueError(f'scale must be positive and finite, got {scale}')
+        out = _out(out, q)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        size = _lib.lib().orc_kv_attend_ws(C.byref(self._c), n, hq, int(prefix_tokens))
+        if size < 0:
+            _lib.check(-1, 'orc_kv_attend_ws')
+        ws = torch.empty(size // 4, dtype=torch.float32, device=self.device) if size else None
+        st = (C.c_int64 * 4)(*_strides(q, 'q'), *_strides(out, 'out'))
+        self._call('orc_kv_attend', int(layer), _ptr(q), _ptr(out), st, r, lim, n, hq, int(prefix_tokens), scale, _ptr(ws))
+        return out
