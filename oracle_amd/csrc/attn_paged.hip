@@ -5,16 +5,23 @@
 // every row's own tokens are read for its n_heads / n_kv_heads query heads. Each part leaves (m, sum, unnormalised output) in fp32;
 // combine_kernel joins the parts of a query by exp2(c (m_part - m)).
 //
-// A workgroup = 4 waves that share 16 QT query columns and split the keys: every wave streams tiles of 32 keys of its own through a 2-deep
-// LDS ring (LDS-DMA, no barrier in the loop), so the loop waits for memory only. Orientation as in attn.hip: S^T = K . Q^T, then
-// O^T = V^T . P^T with the lane's own probabilities as the B operand and V^T by the transposing LDS read.
+// Two shapes of work, 4 waves each:
+//   keys_item  few query columns (16 or 32: one row's heads over its own tokens, or a small batch over the prefix): the waves share the columns and
+//              split the keys. A wave's tile is 32 keys, K straight to registers in operand order, V through 8 KiB of LDS of its own; no
+//              barrier in the loop and little LDS, so 4 workgroups fit a CU and hide each other's memory latency. Bound by HBM.
+//   cols_item  many columns over the prefix: every wave has 32 columns of its own, 64-key tiles go through a 2-deep LDS ring that
+//              the waves share (flash32.h). Bound by the matrix cores and the softmax between the two products.
+// The page ids of an item's keys are gathered into LDS first, so that the loop's addresses wait for no dependent load.
+#include <type_traits>
+
 #include "../../include/oracle_hip.h"
+#include "flash32.h"
 #include "kernels.h"
-#include "mma16.h"
 
 namespace {
 
-constexpr int KT = 32;            // keys of a wave's tile
+constexpr int KT = 32;            // keys of a wave's tile in keys_item
+constexpr int NID = 512;          // page ids held in LDS at a time
 constexpr int MAX_PARTS = 64;     // parts of one query (a lane of the combining wave each)
 
 struct AttendArgs {
@@ -29,8 +36,8 @@ struct AttendArgs {
   float c;
 };
 
-template <int HD> __device__ __forceinline__ int swz_k(int key, int ch) { return HD == 128 ? ch ^ (key & 15) : ch ^ ((key >> 1) & 7); }
-template <int HD> __device__ __forceinline__ int swz_v(int key, int ch) {
+// places of the 16-byte chunks of a V row in keys_item's tile: the 8 keys x 32 bytes of half a transposing read fall on different banks
+template <int HD> __device__ __forceinline__ int swz_v16(int key, int ch) {
   return HD == 128 ? ch ^ ((key & 7) << 1) : ch ^ (((key >> 1) & 3) << 1);
 }
 
@@ -61,95 +68,55 @@ __device__ __forceinline__ int prefix_row(const AttendArgs& a, int lane) {
   return r >= 0 && r < a.max_rows ? r : -1;
 }
 
-template <typename T, int HD, int QT>
-__global__ __launch_bounds__(256, 1) void attend_kernel(AttendArgs a) {
-  typedef typename Mma<T>::v8 v8;
-  constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, STAGE = 2 * TILE, RND = TILE / 1024, KPR = 64 / CH, MT = 16 * QT;
-  constexpr int RING = 4 * 2 * STAGE, JOIN = (8 * MT + 4 * MT * HD) * 4;
-  __shared__ __attribute__((aligned(16))) char smem[RING > JOIN ? RING : JOIN];   // 4 waves x 2 stages x (K | V); afterwards the waves' sums
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
-  const int ps = 1 << a.log_ps, n_pre = a.hkv * a.mt * a.sp;
-  int kvh, part, k_lo, k_hi, row, f0;   // f0: first of the item's query columns; a column is (query, head of the group)
-  int cols;
-  const bool pre = (int)blockIdx.x < n_pre;
-  if (pre) {
-    const int pairs = a.hkv * a.sp, pair = blockIdx.x % pairs, mt = blockIdx.x / pairs;   // column tiles of one key range: one XCD where pairs % 8 == 0
-    kvh = pair % a.hkv;
-    part = pair / a.hkv;
-    const int per = ((a.prefix + KT - 1) / KT + a.sp - 1) / a.sp * KT;
-    k_lo = part * per;
-    k_hi = k_lo + per < a.prefix ? k_lo + per : a.prefix;
-    row = prefix_row(a, lane);
-    f0 = mt * MT;
-    cols = a.n * a.group - f0;
-  } else {
-    int x = blockIdx.x - n_pre;
-    kvh = x % a.hkv; x /= a.hkv;
-    const int gt = x % a.gt; x /= a.gt;
-    const int sx = x % a.ss, i = x / a.ss;
-    const int lim = visible(a, i, &row);
-    if (a.prefix && kvh == 0 && gt == 0 && sx == 0 && w == 0 && row >= 0) {   // what it reads as shared, is it the same pages?
-      const int pr = prefix_row(a, lane), held = ((lim < a.prefix ? lim : a.prefix) + ps - 1) >> a.log_ps;
-      bool differ = false;
-      for (int j = lane; j < held; j += 64) differ |= pr < 0 || a.table[(size_t)row * a.width + j] != a.table[(size_t)pr * a.width + j];
-      if (__any(differ) && lane == 0) atomicOr(a.status, (int)ORC_KV_NOT_SHARED);
-    }
-    const int tiles = (lim - a.prefix + KT - 1) / KT;
-    int per = (tiles + a.ss - 1) / a.ss;
-    per = (per < 4 ? 4 : per) * KT;   // at least a tile for each wave
-    k_lo = a.prefix + sx * per;
-    k_hi = k_lo + per < lim ? k_lo + per : lim;
-    part = a.sp + sx;
-    f0 = i * a.group + gt * MT;
-    cols = a.group - gt * MT;
-  }
-  if (cols > MT) cols = MT;
-  const int nq = (cols + 15) >> 4;
+// What a workgroup does: the keys [k_lo, k_hi) of row `row` for `cols` query columns of K/V head kvh, from column f0 (query, head of the group) on
+struct Item { int kvh, part, k_lo, k_hi, row, f0, cols; };
 
-  // the lane's query columns: c16 of every block of 16
-  int lim_c[QT];
+// ids[e] = page of the tokens [(first + e) ps, ...) of the row, -1 outside the pool; by the whole workgroup
+__device__ __forceinline__ void load_ids(const AttendArgs& a, int row, int first, int count, int* ids) {
+  __syncthreads();
+  for (int e = threadIdx.x; e < count; e += 256) {
+    const int p = row < 0 ? -1 : a.table[(size_t)row * a.width + first + e];
+    ids[e] = p < a.n_pages ? p : -1;
+  }
+  __syncthreads();
+}
+
+// One part of one column's result: m, sum and the output sums of dims d..d+3 (want_ml: by the caller that holds d == 0); the result itself where the
+// column has no other part.
+template <typename T, int HD>
+__device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col, int d, float m, float sum, f32x4 v) {
+  const int f = it.f0 + col, i = f / a.group, head = it.kvh * a.group + f % a.group;
+  if (a.sp + a.ss == 1) {
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    u32x2 st = {cvt2<T>(v[0] * inv, v[1] * inv), cvt2<T>(v[2] * inv, v[3] * inv)};
+    if (sum == 0.f) st = u32x2{0, 0};
+    *(u32x2*)((T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + d) = st;
+  } else {
+    const size_t at = ((size_t)i * a.hq + head) * (a.sp + a.ss) + it.part;
+    if (d == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = sum; }
+    if (sum != 0.f) *(f32x4*)(a.po + at * HD + d) = v;
+  }
+}
+
+template <typename T, int HD, int QT>
+__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, char* smem, int* ids) {
+  typedef typename Mma<T>::v8 v8;
+  constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH, MT = 16 * QT;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
+  const int ps = 1 << a.log_ps, nq = (it.cols + 15) >> 4;
+  int lim_c[QT];                  // the lane's query columns: c16 of every block of 16
   v8 qf[QT][HD / 32];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int col = t * 16 + c16;
-    lim_c[t] = 0;
-    const int f = f0 + (col < cols ? col : 0), i = f / a.group, head = kvh * a.group + f % a.group;
-    if (col < cols) {
-      int r;
-      const int lim = visible(a, i, &r);
-      lim_c[t] = lim < k_hi ? lim : k_hi;
-    }
+    const int f = it.f0 + (col < it.cols ? col : 0), i = f / a.group, head = it.kvh * a.group + f % a.group;
+    int r;
+    const int lim = visible(a, i, &r);
+    lim_c[t] = col < it.cols ? (lim < it.k_hi ? lim : it.k_hi) : 0;
     const T* qp = (const T*)a.q + (size_t)i * a.q_ts + (size_t)head * a.q_hs + g * 8;
 #pragma unroll
     for (int kk = 0; kk < HD / 32; ++kk) qf[t][kk] = *(const v8*)(qp + kk * 32);
   }
-
-  const T* kb = (const T*)a.k + (size_t)kvh * ps * HD;
-  const T* vb = (const T*)a.v + (size_t)kvh * ps * HD;
-  char* ring = smem + w * 2 * STAGE;
-  const int key_p = lane / CH, ch_p = lane % CH;
-  // Pages of a tile's two halves of 16 keys. A page outside the pool: the half is not attended, and its lanes load a token of the other half.
-  auto page_of = [&](int k0) {
-    int p = -1;
-    if (row >= 0 && k0 < k_hi) p = a.table[(size_t)row * a.width + (k0 >> a.log_ps)];
-    p = __builtin_amdgcn_readfirstlane(p);
-    return p < a.n_pages ? p : -1;
-  };
-  auto dma = [&](int k0, int p0, int p1, int stage) {
-    char* sk = ring + stage * STAGE;
-    const int last = k_hi - 1;
-#pragma unroll
-    for (int r = 0; r < RND; ++r) {
-      const int key = r * KPR + key_p;
-      int at = k0 + key, page = key < 16 ? p0 : p1;
-      if (page < 0) { page = key < 16 ? p1 : p0; at = key < 16 ? k0 + 16 : k0; }
-      if (at > last) { at = last; page = (last - k0) < 16 ? p0 : p1; if (page < 0) { page = p0; at = k0; } }
-      const size_t off = (size_t)page * a.page_elems + (size_t)(at & (ps - 1)) * HD;
-      __builtin_amdgcn_global_load_lds((glb_void_t*)(kb + off + swz_k<HD>(key, ch_p) * 8), (lds_void_t*)(sk + r * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_void_t*)(vb + off + swz_v<HD>(key, ch_p) * 8), (lds_void_t*)(sk + TILE + r * 1024), 16, 0, 0);
-    }
-  };
-
   f32x4 o[QT][HD / 16];
   float m[QT], l[QT];
 #pragma unroll
@@ -158,93 +125,96 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  // tiles w, w + 4, ... of the range; a tile none of whose pages is in the pool is passed over
-  int k0 = k_lo + w * KT, p0 = -1, p1 = -1;
-  auto seek = [&](int from) {
-    for (; from < k_hi; from += 4 * KT) {
-      p0 = page_of(from);
-      p1 = page_of(from + 16);
-      if (p0 >= 0 || p1 >= 0) break;
-    }
-    return from;
-  };
-  k0 = seek(k0);
-  if (k0 < k_hi) dma(k0, p0, p1, 0);
-  int stage = 0;
-  while (k0 < k_hi) {
-    const bool ok0 = p0 >= 0, ok1 = p1 >= 0;
-    const int nx = seek(k0 + 4 * KT);
-    if (nx < k_hi) {
-      dma(nx, p0, p1, stage ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * RND) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    const char* sK = ring + stage * STAGE;
-    const char* sV = sK + TILE;
-    f32x4 s[QT][2];
+  const T* kb = (const T*)a.k + (size_t)it.kvh * ps * HD + g * 8;
+  const T* vb = (const T*)a.v + (size_t)it.kvh * ps * HD;
+  char* sV = smem + w * TILE;
+  const int key_p = lane / CH, ch_p = lane % CH;
+  for (int kc = it.k_lo; kc < it.k_hi; kc += (NID - 2) << a.log_ps) {
+    const int first = kc >> a.log_ps, ke = kc + ((NID - 2) << a.log_ps) < it.k_hi ? kc + ((NID - 2) << a.log_ps) : it.k_hi;
+    load_ids(a, it.row, first, ((ke - 1) >> a.log_ps) - first + 1, ids);
+    for (int k0 = kc + w * KT; k0 < ke; k0 += 4 * KT) {
+      // the tile's two halves of 16 keys; one that is not there (behind the end, or its page outside the pool) loads a token of the other
+      const int i0 = (k0 >> a.log_ps) - first, i1 = k0 + 16 < ke ? ((k0 + 16) >> a.log_ps) - first : i0;
+      const int p0 = __builtin_amdgcn_readfirstlane(ids[i0]), p1 = k0 + 16 < ke ? __builtin_amdgcn_readfirstlane(ids[i1]) : -1;
+      if (p0 < 0 && p1 < 0) continue;
+      auto place = [&](int key) {   // element offset of a token of the tile
+        const bool up = key >= 16, there = up ? p1 >= 0 : p0 >= 0;
+        int at = k0 + key < ke ? k0 + key : ke - 1;
+        const int page = (up == there) ? p1 : p0;
+        if (!there) at = up ? k0 : k0 + 16;
+        return (size_t)page * a.page_elems + (size_t)((at & (ps - 1)) * HD);
+      };
+      v8 kf[2][HD / 32];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b) {
+        const T* kp = kb + place(b * 16 + c16);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) s[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int key = b * 16 + c16;
+        for (int kk = 0; kk < HD / 32; ++kk) kf[b][kk] = *(const v8*)(kp + kk * 32);
+      }
 #pragma unroll
-      for (int kk = 0; kk < HD / 32; ++kk) {
-        const v8 kf = *(const v8*)(sK + key * ROWB + (swz_k<HD>(key, kk * 4 + g) << 4));
+      for (int r = 0; r < RND; ++r) {
+        const int key = r * KPR + key_p;
+        __builtin_amdgcn_global_load_lds((glb_void_t*)(vb + place(key) + swz_v16<HD>(key, ch_p) * 8), (lds_void_t*)(sV + r * 1024), 16, 0, 0);
+      }
+      f32x4 s[QT][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            if (t < nq) s[t][b] = Mma<T>::m16(kf[b][kk], qf[t][kk], s[t][b]);
+      }
+      v8 pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        if (t >= nq) continue;
+        float tm = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool see = k0 + b * 16 + 4 * g + r < lim_c[t] && (b ? p1 : p0) >= 0;
+            s[t][b][r] = see ? s[t][b][r] : -INFINITY;
+            tm = fmaxf(tm, s[t][b][r]);
+          }
+        tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+        tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+        const float m_new = fmaxf(m[t], tm), mu = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f((m[t] - mu) * a.c);
+        m[t] = m_new;
+        l[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[t][d] *= alpha;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f((s[t][j >> 2][j & 3] - mu) * a.c);
+          l[t] += p[j];
+        }
+        pf[t] = __builtin_bit_cast(v8, (u32x4){cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])});
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // V is in LDS
+      const int key = 4 * g + (c16 >> 2);
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        const int ch = d * 2 + ((lane & 3) >> 1);
+        const u32x2 v0 = lds_tr16<T>(sV + key * ROWB + (swz_v16<HD>(key, ch) << 4) + (lane & 1) * 8);
+        const u32x2 v1 = lds_tr16<T>(sV + (key + 16) * ROWB + (swz_v16<HD>(key + 16, ch) << 4) + (lane & 1) * 8);
+        const v8 vf = join8<T>(v0, v1);
 #pragma unroll
         for (int t = 0; t < QT; ++t)
-          if (t < nq) s[t][b] = Mma<T>::m16(kf, qf[t][kk], s[t][b]);
+          if (t < nq) o[t][d] = Mma<T>::m16(vf, pf[t], o[t][d]);
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile's reads are done before the next tile's DMA
     }
-    v8 pf[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if (t >= nq) continue;
-      float tm = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool see = k0 + b * 16 + 4 * g + r < lim_c[t] && (b ? ok1 : ok0);
-          s[t][b][r] = see ? s[t][b][r] : -INFINITY;
-          tm = fmaxf(tm, s[t][b][r]);
-        }
-      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-      tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-      const float m_new = fmaxf(m[t], tm), mu = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f((m[t] - mu) * a.c);
-      m[t] = m_new;
-      l[t] *= alpha;
-#pragma unroll
-      for (int d = 0; d < HD / 16; ++d) o[t][d] *= alpha;
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f((s[t][j >> 2][j & 3] - mu) * a.c);
-        l[t] += p[j];
-      }
-      pf[t] = __builtin_bit_cast(v8, (u32x4){cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])});
-    }
-    const int key = 4 * g + (c16 >> 2);
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) {
-      const int ch = d * 2 + ((lane & 3) >> 1);
-      const u32x2 v0 = lds_tr16<T>(sV + key * ROWB + (swz_v<HD>(key, ch) << 4) + (lane & 1) * 8);
-      const u32x2 v1 = lds_tr16<T>(sV + (key + 16) * ROWB + (swz_v<HD>(key + 16, ch) << 4) + (lane & 1) * 8);
-      const v8 vf = join8<T>(v0, v1);
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-        if (t < nq) o[t][d] = Mma<T>::m16(vf, pf[t], o[t][d]);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage's reads are done before the next pass's DMA goes into it
-    stage ^= 1;
-    k0 = nx;
   }
 
-  // join the four waves
+  // join the four waves: maxima and sums of all, then the outputs of waves 2, 3 into 0, 1 and of 1 into 0
   __syncthreads();
-  float* sm = (float*)smem;                  // [4][MT] maxima, [4][MT] sums, then [4][MT][HD]
+  float* sm = (float*)smem;                  // [4][MT] maxima, [4][MT] sums, then [2][MT][HD]
   float* so = sm + 8 * MT;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -253,40 +223,194 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(AttendArgs a) {
     if (g == 0) { sm[w * MT + t * 16 + c16] = m[t]; sm[(4 + w) * MT + t * 16 + c16] = l[t]; }
   }
   __syncthreads();
+  float mx[QT], sum[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int col = t * 16 + c16;
-    float mx = -INFINITY;
-    for (int x = 0; x < 4; ++x) mx = fmaxf(mx, sm[x * MT + col]);
-    const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - mx) * a.c);
-    const bool any = l[t] != 0.f;
+    mx[t] = -INFINITY; sum[t] = 0.f;
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d)
-      *(f32x4*)(so + ((size_t)w * MT + col) * HD + d * 16 + 4 * g) = any ? o[t][d] * f : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  __syncthreads();
-  const int parts = a.sp + a.ss;
-  for (int x = threadIdx.x; x < cols * (HD / 4); x += 256) {
-    const int col = x / (HD / 4), d4 = x % (HD / 4);
-    float mx = -INFINITY, sum = 0.f;
-    for (int y = 0; y < 4; ++y) mx = fmaxf(mx, sm[y * MT + col]);
-    for (int y = 0; y < 4; ++y) {
-      const float my = sm[y * MT + col], ly = sm[(4 + y) * MT + col];
-      if (ly != 0.f) sum += ly * __builtin_amdgcn_exp2f((my - mx) * a.c);
+    for (int x = 0; x < 4; ++x) mx[t] = fmaxf(mx[t], sm[x * MT + col]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float lx = sm[(4 + x) * MT + col];
+      if (lx != 0.f) sum[t] += lx * __builtin_amdgcn_exp2f((sm[x * MT + col] - mx[t]) * a.c);
     }
-    f32x4 v = *(const f32x4*)(so + (size_t)col * HD + d4 * 4);
-    for (int y = 1; y < 4; ++y) v += *(const f32x4*)(so + ((size_t)y * MT + col) * HD + d4 * 4);
-    const int f = f0 + col, i = f / a.group, head = kvh * a.group + f % a.group;
-    if (parts == 1) {
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      u32x2 st = {cvt2<T>(v[0] * inv, v[1] * inv), cvt2<T>(v[2] * inv, v[3] * inv)};
-      *(u32x2*)((T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + d4 * 4) = st;
-    } else {
-      const size_t at = ((size_t)i * a.hq + head) * parts + part;
-      if (d4 == 0) { a.ml[2 * at] = mx; a.ml[2 * at + 1] = sum; }
-      if (sum != 0.f) *(f32x4*)(a.po + at * HD + d4 * 4) = v;
+    const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - mx[t]) * a.c);
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) o[t][d] = l[t] != 0.f ? o[t][d] * f : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int half = 2; half >= 1; half >>= 1) {
+    if (w >= half && w < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) *(f32x4*)(so + (size_t)((w - half) * MT + t * 16 + c16) * HD + d * 16 + 4 * g) = o[t][d];
+    }
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[t][d] += *(const f32x4*)(so + (size_t)(w * MT + t * 16 + c16) * HD + d * 16 + 4 * g);
+    }
+    __syncthreads();
+  }
+  if (w == 0) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+      if (t * 16 + c16 < it.cols)
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) put<T, HD>(a, it, t * 16 + c16, d * 16 + 4 * g, mx[t], sum[t], o[t][d]);
+  }
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, char* smem, int* ids) {
+  typedef Tile64<HD> Tile;
+  constexpr int KB = 64, RND = KB * Tile::CH / 256, KPR = 256 / Tile::CH;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int ps = 1 << a.log_ps, col = w * 32 + (lane & 31);
+  const bool mine = w * 32 < it.cols;          // the wave has columns
+  Flash32<T, HD> f;
+  int lim = it.k_hi;
+  {
+    const int fc = it.f0 + (col < it.cols ? col : 0), i = fc / a.group;
+    f.init((const T*)a.q + (size_t)i * a.q_ts + (size_t)(it.kvh * a.group + fc % a.group) * a.q_hs, lane);
+    int r;
+    const int v = visible(a, i, &r);
+    if (col < it.cols && v < lim) lim = v;
+  }
+  int lim_min = lim;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int y = __shfl_xor(lim_min, x, 64);
+    lim_min = y < lim_min ? y : lim_min;
+  }
+  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+  const T* kb = (const T*)a.k + (size_t)it.kvh * ps * HD;
+  const T* vb = (const T*)a.v + (size_t)it.kvh * ps * HD;
+  const int key_p = tid / Tile::CH, ch_p = tid % Tile::CH;
+  const int ck = Tile::swz_k(key_p, ch_p) * 8, cv = Tile::swz_v(key_p, ch_p) * 8;
+  for (int kc = it.k_lo; kc < it.k_hi; kc += (NID - 4) << a.log_ps) {
+    const int first = kc >> a.log_ps, ke = kc + ((NID - 4) << a.log_ps) < it.k_hi ? kc + ((NID - 4) << a.log_ps) : it.k_hi;
+    load_ids(a, it.row, first, ((ke - 1) >> a.log_ps) - first + 1, ids);
+    // pages of the tile's four units of 16 keys (-1: behind the end, or outside the pool); the first of those that are there, -1 without any
+    int pg[4];
+    auto units = [&](int k0) {
+      int good = -1;
+#pragma unroll
+      for (int u = 3; u >= 0; --u) {
+        pg[u] = k0 + 16 * u < ke ? __builtin_amdgcn_readfirstlane(ids[((k0 + 16 * u) >> a.log_ps) - first]) : -1;
+        if (pg[u] >= 0) good = u;
+      }
+      return good;
+    };
+    auto seek = [&](int k0, int* good) {   // the next tile with a page in the pool
+      for (; k0 < ke; k0 += KB)
+        if ((*good = units(k0)) >= 0) break;
+      return k0;
+    };
+    auto dma = [&](int k0, int good, int stage) {
+      char* sk = smem + stage * 2 * Tile::BYTES + w * 1024;
+#pragma unroll
+      for (int r = 0; r < RND; ++r) {
+        const int pu = HD == 128 ? pg[r] : w >> 1 ? pg[(2 * r + 1) & 3] : pg[(2 * r) & 3];   // page of this wave's keys in this round
+        int at = k0 + r * KPR + key_p, page = pu;
+        if (at >= ke) at = ke - 1;           // behind the last token: that token again, its score is masked
+        if (pu < 0) { page = good == 0 ? pg[0] : good == 1 ? pg[1] : good == 2 ? pg[2] : pg[3]; at = k0 + 16 * good; }
+        const size_t off = (size_t)page * a.page_elems + (size_t)((at & (ps - 1)) * HD);
+        __builtin_amdgcn_global_load_lds((glb_void_t*)(kb + off + ck), (lds_void_t*)(sk + r * 4096), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void_t*)(vb + off + cv), (lds_void_t*)(sk + Tile::BYTES + r * 4096), 16, 0, 0);
+      }
+    };
+    int good;
+    int k0 = seek(kc, &good);
+    if (k0 < ke) dma(k0, good, 0);
+    auto step = [&](auto st) {
+      constexpr int stage = decltype(st)::value;
+      const int now = k0;
+      const unsigned there = (pg[0] >= 0) | (pg[1] >= 0) << 1 | (pg[2] >= 0) << 2 | (pg[3] >= 0) << 3;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      k0 = seek(k0 + KB, &good);
+      if (k0 < ke) dma(k0, good, stage ^ 1);
+      if (!mine) return;
+      const char* sK = smem + stage * 2 * Tile::BYTES;
+      f32x16 s[2];
+      f.scores(sK, s);
+      if (there != 15u || now + KB > lim_min) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = Flash32<T, HD>::key_of(b, i, h);
+            if (now + key >= lim || !(there >> (b * 2 + (i >> 3)) & 1)) s[b][i] = -INFINITY;
+          }
+      }
+      f.add(sK + Tile::BYTES, s, a.c);
+    };
+    while (k0 < ke) {
+      step(std::integral_constant<int, 0>());
+      if (k0 < ke) step(std::integral_constant<int, 1>());
     }
   }
+  const float sum = f.total();
+  if (col < it.cols) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        put<T, HD>(a, it, col, dt * 32 + 2 * i + 4 * h, f.m, sum, f32x4{f.o[dt][i], f.o[dt][i + 1], f.o[dt][i + 2], f.o[dt][i + 3]});
+  }
+}
+
+// PRE: how the prefix is read. 1, 2: keys_item with that many blocks of 16 columns; 8: cols_item, 128 columns
+template <typename T, int HD, int PRE>
+__global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArgs a) {
+  constexpr int QT = PRE == 8 ? 1 : PRE, MT = 16 * PRE;
+  constexpr int V_TILES = 4 * KT * HD * 2, JOIN = (8 + 2 * HD) * 16 * QT * 4, COLS = PRE == 8 ? 4 * Tile64<HD>::BYTES : 0;
+  constexpr int BYTES = V_TILES > JOIN ? (V_TILES > COLS ? V_TILES : COLS) : (JOIN > COLS ? JOIN : COLS);
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  __shared__ int ids[NID];
+  const int lane = threadIdx.x & 63, n_pre = a.hkv * a.mt * a.sp;
+  Item it;
+  if ((int)blockIdx.x < n_pre) {
+    const int pairs = a.hkv * a.sp, pair = blockIdx.x % pairs, mt = blockIdx.x / pairs;   // column tiles of one key range: one XCD where pairs % 8 == 0
+    it.kvh = pair % a.hkv;
+    it.part = pair / a.hkv;
+    const int per = ((a.prefix + KT - 1) / KT + a.sp - 1) / a.sp * KT;
+    it.k_lo = it.part * per;
+    it.k_hi = it.k_lo + per < a.prefix ? it.k_lo + per : a.prefix;
+    it.row = prefix_row(a, lane);
+    it.f0 = mt * MT;
+    it.cols = a.n * a.group - it.f0;
+    if (it.cols > MT) it.cols = MT;
+    if constexpr (PRE == 8) cols_item<T, HD>(a, it, smem, ids);
+    else keys_item<T, HD, QT>(a, it, smem, ids);
+    return;
+  }
+  int x = blockIdx.x - n_pre;
+  it.kvh = x % a.hkv; x /= a.hkv;
+  const int gt = x % a.gt; x /= a.gt;
+  const int sx = x % a.ss, i = x / a.ss;
+  const int lim = visible(a, i, &it.row);
+  if (a.prefix && it.kvh == 0 && gt == 0 && sx == 0 && threadIdx.x < 64 && it.row >= 0) {   // what it reads as shared, is it on the same pages?
+    const int pr = prefix_row(a, lane), held = ((lim < a.prefix ? lim : a.prefix) + (1 << a.log_ps) - 1) >> a.log_ps;
+    bool differ = false;
+    for (int j = lane; j < held; j += 64) differ |= pr < 0 || a.table[(size_t)it.row * a.width + j] != a.table[(size_t)pr * a.width + j];
+    if (__any(differ) && lane == 0) atomicOr(a.status, (int)ORC_KV_NOT_SHARED);
+  }
+  const int tiles = (lim - a.prefix + KT - 1) / KT;
+  int per = (tiles + a.ss - 1) / a.ss;
+  per = (per < 4 ? 4 : per) * KT;   // at least a tile for each wave
+  it.k_lo = a.prefix + sx * per;
+  it.k_hi = it.k_lo + per < lim ? it.k_lo + per : lim;
+  it.part = a.sp + sx;
+  it.f0 = i * a.group + gt * 16;
+  it.cols = a.group - gt * 16;
+  if (it.cols > 16) it.cols = 16;
+  keys_item<T, HD, 1>(a, it, smem, ids);
 }
 
 // one wave per (query, head): lane s holds part s
@@ -320,19 +444,18 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
 }
 
 // how a call is split; the same for the scratch size and the launch
-struct Split { int qt, mt, gt, sp, ss; };
+struct Split { int pre, mt, gt, sp, ss; };
 Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   Split s;
   const int group = n_heads / c->n_kv_heads;
   const int64_t cols = (int64_t)n * group;
-  const int64_t most = prefix ? cols : group;
-  s.qt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-  s.mt = prefix ? (int)((cols + 16 * s.qt - 1) / (16 * s.qt)) : 0;
-  s.gt = (group + 16 * s.qt - 1) / (16 * s.qt);
+  s.pre = cols <= 16 ? 1 : cols <= 32 ? 2 : 8;
+  s.mt = prefix ? (int)((cols + 16 * s.pre - 1) / (16 * s.pre)) : 0;
+  s.gt = (group + 15) / 16;
   s.sp = 0;
   if (prefix) {
     const int64_t base = (int64_t)c->n_kv_heads * s.mt;
-    int64_t sp = (512 + base - 1) / base;
+    int64_t sp = 512 / base;
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
     s.sp = (int)(sp < 1 ? 1 : sp > 32 ? 32 : sp);
@@ -357,15 +480,15 @@ const char* bad_call(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   return nullptr;
 }
 
-template <typename T, int HD, int QT> hipError_t launch_qt(const AttendArgs& a, hipStream_t s) {
+template <typename T, int HD, int PRE> hipError_t launch_pre(const AttendArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)(a.hkv * a.mt * a.sp + a.n * a.hkv * a.gt * a.ss);
-  hipLaunchKernelGGL((attend_kernel<T, HD, QT>), dim3(grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attend_kernel<T, HD, PRE>), dim3(grid), dim3(256), 0, s, a);
   if (a.sp + a.ss > 1)
     hipLaunchKernelGGL((combine_kernel<T, HD>), dim3((unsigned)(((int64_t)a.n * a.hq + 3) / 4)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
-template <typename T, int HD> hipError_t launch_hd(const AttendArgs& a, int qt, hipStream_t s) {
-  return qt == 1 ? launch_qt<T, HD, 1>(a, s) : qt == 2 ? launch_qt<T, HD, 2>(a, s) : launch_qt<T, HD, 4>(a, s);
+template <typename T, int HD> hipError_t launch_hd(const AttendArgs& a, int pre, hipStream_t s) {
+  return pre == 1 ? launch_pre<T, HD, 1>(a, s) : pre == 2 ? launch_pre<T, HD, 2>(a, s) : launch_pre<T, HD, 8>(a, s);
 }
 
 }  // namespace
@@ -408,7 +531,7 @@ extern "C" int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, vo
   a.c = scale * 1.4426950408889634f;
   hipStream_t hs = (hipStream_t)stream;
   hipError_t e;
-  if (c->dtype == 0) e = c->head_dim == 128 ? launch_hd<__bf16, 128>(a, s.qt, hs) : launch_hd<__bf16, 64>(a, s.qt, hs);
-  else e = c->head_dim == 128 ? launch_hd<_Float16, 128>(a, s.qt, hs) : launch_hd<_Float16, 64>(a, s.qt, hs);
+  if (c->dtype == 0) e = c->head_dim == 128 ? launch_hd<__bf16, 128>(a, s.pre, hs) : launch_hd<__bf16, 64>(a, s.pre, hs);
+  else e = c->head_dim == 128 ? launch_hd<_Float16, 128>(a, s.pre, hs) : launch_hd<_Float16, 64>(a, s.pre, hs);
   return e == hipSuccess ? 0 : orc_fail(who, hipGetErrorString(e));
 }

@@ -1,0 +1,96 @@
+// One wave's part of attention over 64-key tiles in LDS: 32 query columns, running maximum, sum and output in registers. Used by the kernels of
+// attn_packed.hip (prompts) and attn_paged.hip (a prefix that many queries share).
+//
+// Orientation (no value crosses lanes between the two products):
+//   S^T = K . Q^T    A = 32 keys x 16 from LDS, B = the wave's 32 query columns held in registers
+//                    -> lane (q = lane & 31, h = lane >> 5) holds keys 8 (i / 4) + 4 h + i % 4 of its query, i = 0..15
+//   O^T = V^T . P^T  the k-slots (h, j) of the product are DEFINED as the keys the lane holds: P is its own registers rounded to 16 bits,
+//                    V^T comes by the transposing LDS read in that order.
+// p = exp2(c (s - m)) with c = scale * log2(e). m is raised (and o, l rescaled, a wave-uniform branch) only where a tile's maximum exceeds it by
+// more than 8 / c: p then stays below 2^8, whose rounding to 16 bits is as exact relatively as below 1, and the 64 multiplies of a
+// rescale are spent on few tiles.
+#pragma once
+#include "mma16.h"
+
+// A tile image: 64 rows (keys) of HD values, 16-byte chunk ch of a row at place swz(key, ch), an involution. The 8 lanes of a ds_read_b128 phase
+// (8 keys, one chunk) and the 4 keys x 64 bytes of half a transposing read then fall on different banks. LDS-DMA writes lane-linearly, so the
+// permutation is applied to the lanes' source addresses.
+template <int HD> struct Tile64 {
+  static constexpr int KEYS = 64, ROWB = HD * 2, CH = HD / 8, BYTES = KEYS * ROWB;
+  static __device__ __forceinline__ int swz_k(int key, int ch) { return HD == 128 ? ch ^ (key & 15) : ch ^ ((key >> 1) & 7); }
+  static __device__ __forceinline__ int swz_v(int key, int ch) { return HD == 128 ? ch ^ ((key & 3) << 2) : ch ^ (((key >> 1) & 1) << 2); }
+};
+
+template <typename T, int HD> struct Flash32 {
+  typedef typename Mma<T>::v8 v8;
+  typedef Tile64<HD> Tile;
+  v8 qf[HD / 16];
+  f32x16 o[HD / 32];
+  float m, l;             // l: over the lane's own keys, the other half's are added in total()
+  int ka[HD / 16], va[HD / 32];   // byte places of the lane's K chunk (keys 0..31) and V piece (keys 0..15) in the tile images
+
+  __device__ __forceinline__ void init(const T* q, int lane) {   // q: the lane's query row
+    const int c32 = lane & 31, h = lane >> 5, vr = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      qf[kk] = *(const v8*)(q + h * 8 + kk * 16);
+      ka[kk] = c32 * Tile::ROWB + (Tile::swz_k(c32, kk * 2 + h) << 4);
+    }
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt) {
+      va[dt] = vr * Tile::ROWB + (Tile::swz_v(vr, dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ void scores(const char* sK, f32x16 (&s)[2]) const {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) s[b] = Mma<T>::m32(*(const v8*)(sK + ka[kk] + b * 32 * Tile::ROWB), qf[kk], s[b]);
+    }
+  }
+  // key of s[b][i] inside the tile
+  static __device__ __forceinline__ int key_of(int b, int i, int h) { return b * 32 + 8 * (i >> 2) + 4 * h + (i & 3); }
+
+  // adds the tile: scores s (masked ones -inf), values at sV
+  __device__ __forceinline__ void add(const char* sV, const f32x16 (&s)[2], float c) {
+    float tm = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[b][i]);
+    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+    if (__any((tm - m) * c > 8.f)) {   // -inf - -inf: a column that has seen no key yet, and sees none here
+      const float m_new = fmaxf(m, tm), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= alpha;
+    }
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    u32x4 pf[4];   // [16-key group][two keys a register]
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], c, -mc));
+        l += p0 + p1;
+        pf[b * 2 + (i >> 3)][(i & 7) >> 1] = cvt2<T>(p0, p1);
+      }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v8 p8 = __builtin_bit_cast(v8, pf[g]);
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; ++dt) {
+        const char* p = sV + va[dt] + g * 16 * Tile::ROWB;
+        o[dt] = Mma<T>::m32(join8<T>(lds_tr16<T>(p), lds_tr16<T>(p + 8 * Tile::ROWB)), p8, o[dt]);
+      }
+    }
+  }
+  __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
+};

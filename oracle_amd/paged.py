@@ -7,7 +7,6 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .engine import _ptr
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ERRORS = ((1, 'a row outside the table'), (2, 'a row named twice (or a fork onto one of its sources)'), (4, 'a bad token count'),
@@ -15,10 +14,20 @@ _ERRORS = ((1, 'a row outside the table'), (2, 'a row named twice (or a fork ont
            (64, 'a page outside the pool'), (128, 'rows that do not share the prefix they were attended with'))
 
 
-def _on(t):
-    """(stream of t's GPU, context that makes that GPU the current one)"""
-    i = t.device.index
-    return C.c_void_p(torch.cuda.current_stream(i).cuda_stream), torch.cuda.device(i)
+_I64x4, _I64x8 = C.c_int64 * 4, C.c_int64 * 8
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _run(device, name, *args):
+    """The C entry `name` with args and the current stream of `device`, with `device` the current one."""
+    fn, i = getattr(_lib.lib(), name), device.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def _chk(t, name, dim, dtype=None, device=None):
@@ -37,10 +46,11 @@ def _chk(t, name, dim, dtype=None, device=None):
 
 def _strides(t, name):
     """(token stride, head stride) of (tokens, heads, head_dim)"""
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    (n, heads, hd), (ts, hs, es) = t.shape, t.stride()
+    if es != 1 and hd > 1:
         raise ValueError(f'{name}: the last dimension must be contiguous')
-    ts, hs = (t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
-    if ts < 0 or hs < 0 or ts % 8 or hs % 8 or t.data_ptr() % 16:
+    ts, hs = ts if n > 1 else 0, hs if heads > 1 else 0
+    if ts % 8 or hs % 8 or t.data_ptr() % 16:
         raise ValueError(f'{name}: token and head strides must be multiples of 8 elements and the tensor must start on 16 bytes, '
                          f'got strides {tuple(t.stride())} at {t.data_ptr() % 16} bytes past 16')
     return ts, hs
@@ -63,7 +73,7 @@ def _ints(t, name, device, n=None):
         raise ValueError(f'{name} must be contiguous')
     if n is not None and t.numel() != n:
         raise ValueError(f'{name} must hold {n} values, got {t.numel()}')
-    return _ptr(t)
+    return t.data_ptr()
 
 
 def _out(out, like, name='out'):
@@ -94,7 +104,7 @@ class PackedPlan:
         if self.n_work < 0:
             _lib.check(self.n_work, 'orc_attn_plan')
         work = torch.empty(max(self.n_work, 1), 4, dtype=torch.int32)
-        if lib.orc_attn_plan(arr, n, self.tile, _ptr(work), self.n_work) < 0:
+        if lib.orc_attn_plan(arr, n, self.tile, work.data_ptr(), self.n_work) < 0:
             _lib.check(-1, 'orc_attn_plan')
         self.work = work.to(device)
 
@@ -123,11 +133,9 @@ def packed_attention(q, k, v, plan, scale=None, out=None):
     out = _out(out, q)
     if out is None:
         out = (torch.empty if plan.total == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-    st = (C.c_int64 * 8)(*_strides(q, 'q'), *_strides(k, 'k'), *_strides(v, 'v'), *_strides(out, 'out'))
-    stream, dev = _on(q)
-    with dev:
-        _lib.check(_lib.lib().orc_attention_packed(_ptr(q), _ptr(k), _ptr(v), _ptr(out), st, _ptr(plan.work), plan.n_work, plan.tile, plan.total,
-                                                   hq, hkv, hd, _DTYPES[q.dtype], scale, stream), 'orc_attention_packed')
+    st = _I64x8(*_strides(q, 'q'), *_strides(k, 'k'), *_strides(v, 'v'), *_strides(out, 'out'))
+    _run(q.device, 'orc_attention_packed', q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, plan.work.data_ptr(), plan.n_work, plan.tile,
+         plan.total, hq, hkv, hd, _DTYPES[q.dtype], scale)
     return out
 
 
@@ -177,11 +185,10 @@ class KvPages:
         self._work = torch.zeros(8 + 4 * n_pages, dtype=torch.int32, device=kv.device)
         self._c = _lib.OrcKvPages(*[t.data_ptr() for t in (kv, table, lens, refs, self.status, self._work)], layers, n_pages, hkv, page, hd,
                                   table.shape[0], table.shape[1], _DTYPES[kv.dtype])
+        self._ref = C.byref(self._c)
 
     def _call(self, name, *args):
-        stream, dev = _on(self.kv)
-        with dev:
-            _lib.check(getattr(_lib.lib(), name)(C.byref(self._c), *args, stream), name)
+        _run(self.device, name, self._ref, *args)
 
     def _rows(self, rows, name='rows', n=None):
         p = _ints(rows, name, self.device, n)
@@ -210,7 +217,7 @@ class KvPages:
         if not 0 <= total <= 1 << 20:
             raise ValueError(f'total must be 0..2^20, got {total}')
         slots = torch.empty(total, dtype=torch.int32, device=self.device)
-        self._call('orc_kv_reserve', r, c, n, _ptr(slots), int(total))
+        self._call('orc_kv_reserve', r, c, n, slots.data_ptr(), int(total))
         return slots
 
     def append(self, layer, slots, k, v):
@@ -221,8 +228,8 @@ class KvPages:
         if tuple(k.shape) != want or tuple(v.shape) != want:
             raise ValueError(f'k {tuple(k.shape)} and v {tuple(v.shape)} must be {want}')
         self._layer(layer)
-        st = (C.c_int64 * 4)(*_strides(k, 'k'), *_strides(v, 'v'))
-        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), slots.numel(), _ptr(k), _ptr(v), st)
+        st = _I64x4(*_strides(k, 'k'), *_strides(v, 'v'))
+        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), slots.numel(), k.data_ptr(), v.data_ptr(), st)
 
     def _layer(self, layer):
         if not 0 <= layer < self.n_layers:
@@ -252,7 +259,7 @@ class KvPages:
         (n_pages may differ), which becomes a copy of this one without the holes; this one stays as it is."""
         if into is not None and into.device != self.device:
             raise ValueError(f'into is on {into.device}, not on {self.device}')
-        self._call('orc_kv_compact', None if into is None else C.byref(into._c))
+        self._call('orc_kv_compact', None if into is None else into._ref)
 
     def attend(self, layer, q, rows, prefix_tokens=0, limits=None, scale=None, out=None):
         """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
@@ -277,10 +284,11 @@ class KvPages:
         out = _out(out, q)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        size = _lib.lib().orc_kv_attend_ws(C.byref(self._c), n, hq, int(prefix_tokens))
+        size = _lib.lib().orc_kv_attend_ws(self._ref, n, hq, int(prefix_tokens))
         if size < 0:
             _lib.check(-1, 'orc_kv_attend_ws')
         ws = torch.empty(size // 4, dtype=torch.float32, device=self.device) if size else None
-        st = (C.c_int64 * 4)(*_strides(q, 'q'), *_strides(out, 'out'))
-        self._call('orc_kv_attend', int(layer), _ptr(q), _ptr(out), st, r, lim, n, hq, int(prefix_tokens), scale, _ptr(ws))
+        st = _I64x4(*_strides(q, 'q'), *_strides(out, 'out'))
+        self._call('orc_kv_attend', int(layer), q.data_ptr(), out.data_ptr(), st, r, lim, n, hq, int(prefix_tokens), scale,
+                   ws.data_ptr() if size else None)
         return out
