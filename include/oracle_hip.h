@@ -187,17 +187,15 @@ int orc_decode_weight_stats(orc_engine* e, int64_t* out6);
  * elements, multiples of 8 (the innermost dimension is contiguous), and every tensor starts on 16 bytes. Asynchronous on
  * `stream`, no allocation, no host synchronisation: every call can be captured into a graph.
  *
- * orc_attn_plan (host only): the query tiles of n sequences that lie one behind the other, lens_host[i] >= 0 tokens each, `bm`
- * query rows per tile, longest key range first; four ints a tile (first token of the sequence, its length, first query row of the tile in it,
- * 0) to out_host. Returns the number of tiles (out_host may be NULL to count them), -1 on error.
- * orc_attn_tile (host only): the tile height to plan for: 128, or 256 where the prompts are long enough to fill the GPU with those.
+ * orc_attn_plan (host only): the query tiles of n sequences that lie one behind the other, lens_host[i] >= 0 tokens each; four ints a
+ * tile (first token of the sequence, its length, first query row of the tile in it, 0) to out_host, in the order they are run. Returns
+ * the number of tiles (out_host may be NULL to count them), -1 on error.
  * orc_attention_packed: causal attention inside every sequence, token t of a sequence over its tokens 0..t.
  * q (total, n_heads, head_dim), k / v (total, n_kv_heads, head_dim), out like q; strides8 = {q token, q head, k token, k head,
  * v token, v head, out token, out head}; work = the plan on the device. Rows of `out` that no sequence covers are left as they are. */
-int orc_attn_plan(const int32_t* lens_host, int n, int bm, int32_t* out_host, int capacity);
-int orc_attn_tile(const int32_t* lens_host, int n, int n_heads);
+int orc_attn_plan(const int32_t* lens_host, int n, int32_t* out_host, int capacity);
 int orc_attention_packed(const void* q, const void* k, const void* v, void* out, const int64_t* strides8, const int32_t* work, int n_work,
-                         int bm, int total, int n_heads, int n_kv_heads, int head_dim, int dtype, float scale, void* stream);
+                         int total, int n_heads, int n_kv_heads, int head_dim, int dtype, float scale, void* stream);
 
 /* A paged KV cache. The caller owns every array (device): kv [n_layers][2 (K, V)][n_pages][n_kv_heads][page_size][head_dim];
  * table [max_rows][max_row_pages], page of every page_size tokens of a row, -1 behind its last page; lens [max_rows] tokens held; refs [n_pages]

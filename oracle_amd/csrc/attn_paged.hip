@@ -337,8 +337,7 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
       if (k0 < ke) dma(k0, good, stage ^ 1);
       if (!mine) return;
       const char* sK = smem + stage * 2 * Tile::BYTES;
-      f32x16 s[2];
-      f.scores(sK, s);
+      f32x16 s[2] = {f.scores(sK, 0), f.scores(sK, 1)};
       if (there != 15u || now + KB > lim_min) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)

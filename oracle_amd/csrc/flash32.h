@@ -45,26 +45,27 @@ template <typename T, int HD> struct Flash32 {
     m = -INFINITY;
     l = 0.f;
   }
-  __device__ __forceinline__ void scores(const char* sK, f32x16 (&s)[2]) const {
+  // scores of keys 32 b .. 32 b + 31 of a tile
+  __device__ __forceinline__ f32x16 scores(const char* sK, int b) const {
+    f32x16 s;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) s[b] = Mma<T>::m32(*(const v8*)(sK + ka[kk] + b * 32 * Tile::ROWB), qf[kk], s[b]);
-    }
+    for (int kk = 0; kk < HD / 16; ++kk) s = Mma<T>::m32(*(const v8*)(sK + ka[kk] + b * 32 * Tile::ROWB), qf[kk], s);
+    return s;
   }
   // key of s[b][i] inside the tile
   static __device__ __forceinline__ int key_of(int b, int i, int h) { return b * 32 + 8 * (i >> 2) + 4 * h + (i & 3); }
 
-  // adds the tile: scores s (masked ones -inf), values at sV
-  __device__ __forceinline__ void add(const char* sV, const f32x16 (&s)[2], float c) {
+  __device__ __forceinline__ float largest(const f32x16 (&s)[2]) const {
     float tm = s[0][0];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[b][i]);
-    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+    return fmaxf(tm, __shfl_xor(tm, 32, 64));
+  }
+  __device__ __forceinline__ void raise(float tm, float c) {   // tm: the tile's maximum
     if (__any((tm - m) * c > 8.f)) {   // -inf - -inf: a column that has seen no key yet, and sees none here
       const float m_new = fmaxf(m, tm), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
       m = m_new;
@@ -72,16 +73,18 @@ template <typename T, int HD> struct Flash32 {
 #pragma unroll
       for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= alpha;
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    u32x4 pf[4];   // [16-key group][two keys a register]
+  }
+  __device__ __forceinline__ float base(float c) const { return m == -INFINITY ? 0.f : -m * c; }
+  // p of 32 keys, mc = base(c); pf: [16-key group][two keys a register]
+  __device__ __forceinline__ void weights(const f32x16& s, float c, float mc, u32x4* pf) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], c, -mc));
-        l += p0 + p1;
-        pf[b * 2 + (i >> 3)][(i & 7) >> 1] = cvt2<T>(p0, p1);
-      }
+    for (int i = 0; i < 16; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, mc));
+      l += p0 + p1;
+      pf[i >> 3][(i & 7) >> 1] = cvt2<T>(p0, p1);
+    }
+  }
+  __device__ __forceinline__ void values(const char* sV, const u32x4 (&pf)[4]) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const v8 p8 = __builtin_bit_cast(v8, pf[g]);
@@ -91,6 +94,15 @@ template <typename T, int HD> struct Flash32 {
         o[dt] = Mma<T>::m32(join8<T>(lds_tr16<T>(p), lds_tr16<T>(p + 8 * Tile::ROWB)), p8, o[dt]);
       }
     }
+  }
+  // adds the tile: scores s (masked ones -inf), values at sV
+  __device__ __forceinline__ void add(const char* sV, const f32x16 (&s)[2], float c) {
+    raise(largest(s), c);
+    u32x4 pf[4];
+    const float mc = base(c);
+    weights(s[0], c, mc, pf);
+    weights(s[1], c, mc, pf + 2);
+    values(sV, pf);
   }
   __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };

@@ -91,7 +91,7 @@ class PackedPlan:
     """The query tiles of prompts that lie one behind the other, `lens` tokens each (0 allowed), on `device`: made once for a batch
     and used for every layer. It holds for any number of heads."""
 
-    def __init__(self, lens, device='cuda', n_heads=32):
+    def __init__(self, lens, device='cuda'):
         self.lens = [int(x) for x in lens]
         n = len(self.lens)
         if any(x < 0 or x > 0x7fffffff for x in self.lens) or sum(self.lens) > 0x7fffffff:
@@ -99,12 +99,11 @@ class PackedPlan:
         self.total = sum(self.lens)
         lib = _lib.lib()
         arr = (C.c_int32 * max(n, 1))(*self.lens)
-        self.tile = lib.orc_attn_tile(arr, n, int(n_heads))
-        self.n_work = lib.orc_attn_plan(arr, n, self.tile, None, 0)
+        self.n_work = lib.orc_attn_plan(arr, n, None, 0)
         if self.n_work < 0:
             _lib.check(self.n_work, 'orc_attn_plan')
         work = torch.empty(max(self.n_work, 1), 4, dtype=torch.int32)
-        if lib.orc_attn_plan(arr, n, self.tile, work.data_ptr(), self.n_work) < 0:
+        if lib.orc_attn_plan(arr, n, work.data_ptr(), self.n_work) < 0:
             _lib.check(-1, 'orc_attn_plan')
         self.work = work.to(device)
 
@@ -134,8 +133,8 @@ def packed_attention(q, k, v, plan, scale=None, out=None):
     if out is None:
         out = (torch.empty if plan.total == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
     st = _I64x8(*_strides(q, 'q'), *_strides(k, 'k'), *_strides(v, 'v'), *_strides(out, 'out'))
-    _run(q.device, 'orc_attention_packed', q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, plan.work.data_ptr(), plan.n_work, plan.tile,
-         plan.total, hq, hkv, hd, _DTYPES[q.dtype], scale)
+    _run(q.device, 'orc_attention_packed', q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, plan.work.data_ptr(), plan.n_work, plan.total,
+         hq, hkv, hd, _DTYPES[q.dtype], scale)
     return out
 
 

@@ -17,45 +17,38 @@ def lib():
 
 
 @pytest.mark.parametrize('lens', [[], [0], [1], [5, 0, 128, 129, 1, 700], [256, 255, 257], [2305] * 3 + [1] * 40])
-@pytest.mark.parametrize('tile', [128, 256])
-def test_plan_covers_every_row_once_and_lists_long_tiles_first(lib, lens, tile):
+def test_plan_covers_every_row_once_and_runs_a_prompts_tiles_together(lib, lens):
     arr = (C.c_int32 * max(len(lens), 1))(*lens)
-    n = lib.orc_attn_plan(arr, len(lens), tile, None, 0)
-    assert n == sum(-(-x // tile) for x in lens)
+    n = lib.orc_attn_plan(arr, len(lens), None, 0)
     work = np.full((n + 1, 4), -7, dtype=np.int32)
-    assert lib.orc_attn_plan(arr, len(lens), tile, work.ctypes.data, n) == n
+    assert lib.orc_attn_plan(arr, len(lens), work.ctypes.data, n) == n
     assert (work[n] == -7).all()
-    rows, cost = [], []
-    starts = np.cumsum([0] + lens)
-    for start, length, q0, _ in work[:n].tolist():
-        assert (start, length) in set(zip(starts.tolist(), lens)) and q0 % tile == 0 and q0 < length
-        rows += range(start + q0, start + min(q0 + tile, length))
-        cost.append(min(q0 + tile, length))
-    assert sorted(rows) == list(range(sum(lens)))
-    assert cost == sorted(cost, reverse=True)
+    starts = np.cumsum([0] + lens).tolist()
+    tile = 128
+    want = [(s, x, q0, 0) for x, s in sorted(zip(lens, starts), key=lambda y: (-y[0], y[1])) for q0 in reversed(range(0, x, tile))]
+    assert [tuple(x) for x in work[:n].tolist()] == want
 
 
 def test_plan_refusals(lib):
     arr = (C.c_int32 * 2)(5, -1)
-    assert lib.orc_attn_plan(arr, 2, 128, None, 0) == -1 and b'negative length' in lib.orc_last_error()
-    assert lib.orc_attn_plan(arr, 1, 96, None, 0) == -1
-    assert lib.orc_attn_plan(None, 1, 128, None, 0) == -1
+    assert lib.orc_attn_plan(arr, 2, None, 0) == -1 and b'negative length' in lib.orc_last_error()
+    assert lib.orc_attn_plan(None, 1, None, 0) == -1
     big = (C.c_int32 * 2)(0x7fffffff, 1)
-    assert lib.orc_attn_plan(big, 2, 128, None, 0) == -1
+    assert lib.orc_attn_plan(big, 2, None, 0) == -1
     out = np.zeros((1, 4), dtype=np.int32)
     two = (C.c_int32 * 2)(5, 5)
-    assert lib.orc_attn_plan(two, 2, 128, out.ctypes.data, 1) == -1 and b'capacity' in lib.orc_last_error()
+    assert lib.orc_attn_plan(two, 2, out.ctypes.data, 1) == -1 and b'capacity' in lib.orc_last_error()
     with pytest.raises(ValueError):
         PackedPlan([3, -1], device='cpu')
     with pytest.raises(ValueError):
         PackedPlan([0x7fffffff, 1], device='cpu')
 
 
-PACKED_OK = dict(st=[1024, 128] * 4, n_work=1, bm=128, total=4, hq=8, hkv=8, hd=128, dtype=0, scale=0.1, ptr=4096)
+PACKED_OK = dict(st=[1024, 128] * 4, n_work=1, total=4, hq=8, hkv=8, hd=128, dtype=0, scale=0.1, ptr=4096)
 
 
 @pytest.mark.parametrize('change, text', [
-    (dict(hq=9), b'multiple'), (dict(hkv=0), b'multiple'), (dict(hd=96), b'head_dim'), (dict(dtype=2), b'dtype'), (dict(bm=64), b'tile'),
+    (dict(hq=9), b'multiple'), (dict(hkv=0), b'multiple'), (dict(hd=96), b'head_dim'), (dict(dtype=2), b'dtype'),
     (dict(scale=0.0), b'scale'), (dict(scale=float('nan')), b'scale'), (dict(scale=-1.0), b'scale'), (dict(scale=float('inf')), b'scale'),
     (dict(st=[1020] + [1024] * 7), b'strides'), (dict(st=[-8] + [1024] * 7), b'strides'), (dict(ptr=0), b'null'), (dict(ptr=4104), b'aligned'),
     (dict(n_work=-1), b'bad'), (dict(n_work=1 << 30), b'too many')])
@@ -63,7 +56,7 @@ def test_packed_attention_refusals_of_the_c_entry(lib, change, text):
     a = dict(PACKED_OK, **change)
     st = (C.c_int64 * 8)(*a['st'])
     p = a['ptr']
-    rc = lib.orc_attention_packed(p, p, p, p, st, p, a['n_work'], a['bm'], a['total'], a['hq'], a['hkv'], a['hd'], a['dtype'], a['scale'], None)
+    rc = lib.orc_attention_packed(p, p, p, p, st, p, a['n_work'], a['total'], a['hq'], a['hkv'], a['hd'], a['dtype'], a['scale'], None)
     assert rc == -1 and text in lib.orc_last_error()
 
 

@@ -67,7 +67,7 @@ def qkv(total, hq, hkv, hd, dtype, seed, qscale=2.0):
 @pytest.mark.parametrize('hq, hkv, hd, dtype', [(4, 4, 128, BF), (8, 2, 64, FP), (6, 1, 128, FP), (16, 8, 64, BF)])
 def test_packed_attention(lens, hq, hkv, hd, dtype):
     q, k, v = qkv(sum(lens), hq, hkv, hd, dtype, 1)
-    out = packed_attention(q, k, v, PackedPlan(lens, n_heads=hq))
+    out = packed_attention(q, k, v, PackedPlan(lens))
     ref, tol = packed64(q, k, v, lens, hd ** -0.5)
     close(out, ref, tol, lens)
 
@@ -76,7 +76,7 @@ def test_packed_attention_long_enough_for_the_tall_tiles():
     lens = [4200, 3900, 77]
     for hd, dtype in ((128, BF), (64, FP)):
         q, k, v = qkv(sum(lens), 16, 2, hd, dtype, 2)
-        out = packed_attention(q, k, v, PackedPlan(lens, n_heads=16), scale=0.11)
+        out = packed_attention(q, k, v, PackedPlan(lens), scale=0.11)
         at = 0
         for n in lens:      # every 53rd token of every prompt
             for t in range(0, n, 53):
@@ -89,7 +89,7 @@ def test_packed_attention_large_scores_and_peaked_rows():
     lens = [300, 41]
     q, k, v = qkv(sum(lens), 4, 4, 128, BF, 3, qscale=40.0)
     k[0] *= 30
-    out = packed_attention(q, k, v, PackedPlan(lens, n_heads=4))
+    out = packed_attention(q, k, v, PackedPlan(lens))
     ref, tol = packed64(q, k, v, lens, 128 ** -0.5)
     close(out, ref, tol, 'peaked')
 
@@ -97,7 +97,7 @@ def test_packed_attention_large_scores_and_peaked_rows():
 def test_packed_attention_rows_behind_and_neighbours_do_not_matter():
     lens = [70, 0, 130]
     q, k, v = qkv(sum(lens) + 9, 4, 2, 128, BF, 4)
-    plan = PackedPlan(lens, n_heads=4)
+    plan = PackedPlan(lens)
     clean = packed_attention(q, k, v, plan)
     assert (clean[200:] == 0).all()
     for poison in (float('nan'), float('inf'), float('-inf'), torch.finfo(BF).min):
@@ -116,7 +116,7 @@ def test_packed_attention_rows_behind_and_neighbours_do_not_matter():
 def test_packed_attention_layouts_stream_and_graph():
     lens = [90, 33]
     q, k, v = qkv(123, 8, 4, 64, FP, 5)
-    plan = PackedPlan(lens, n_heads=8)
+    plan = PackedPlan(lens)
     want = packed_attention(q, k, v, plan)
     heads_first = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)      # noqa: E731
     out = torch.empty(8, 123, 64, dtype=FP, device=DEV).transpose(0, 1)
@@ -140,7 +140,7 @@ def test_packed_attention_layouts_stream_and_graph():
 
 def test_packed_attention_refusals():
     q, k, v = qkv(16, 4, 2, 64, BF, 6)
-    plan = PackedPlan([16], n_heads=4)
+    plan = PackedPlan([16])
     for bad in ((q.float(), k, v), (q, k.to(FP), v), (q, k[:8], v), (q, k, v[:, :1]), (q[:, :3], k, v), (q[..., :32], k[..., :32], v[..., :32]),
                 (q[:8], k[:8], v[:8]), (q[0], k, v), (q.cpu(), k, v), (q.transpose(1, 2).contiguous().transpose(1, 2), k, v)):
         with pytest.raises(ValueError):
@@ -543,7 +543,7 @@ def test_frames_and_questions_together():
     lens = [150, 96]                                      # two frames
     c = KvPages(layers, 40, hkv, hd, page_size=page, max_rows=10, max_row_pages=8)
     dense = {r: [([], []) for _ in range(layers)] for r in range(10)}
-    plan = PackedPlan(lens, n_heads=hq)
+    plan = PackedPlan(lens)
     slots = c.reserve(ints([0, 1]), ints(lens), total=sum(lens))
     for layer in range(layers):
         q, k, v = qkv(sum(lens), hq, hkv, hd, BF, 30 + layer)
