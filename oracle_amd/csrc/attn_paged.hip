@@ -41,15 +41,16 @@ template <int HD> __device__ __forceinline__ int swz_v16(int key, int ch) {
   return HD == 128 ? ch ^ ((key & 7) << 1) : ch ^ (((key >> 1) & 3) << 1);
 }
 
-// tokens of row rows[i] that query i reads; *row: that row, -1 where it is outside the table
+// tokens of row rows[i] that query i reads; *row: that row, -1 where it is outside the table. No branch, so that other loads need not wait.
 __device__ __forceinline__ int visible(const AttendArgs& a, int i, int* row) {
-  const int r = a.rows[i];
-  *row = r >= 0 && r < a.max_rows ? r : -1;
-  if (*row < 0) return 0;
-  int lim = a.lens[r];
-  if (a.limits && a.limits[i] < lim) lim = a.limits[i];
-  const int cap = a.width << a.log_ps;
-  return lim < 0 ? 0 : lim > cap ? cap : lim;
+  const int r = a.rows[i], cap = a.width << a.log_ps;
+  const bool ok = r >= 0 && r < a.max_rows;
+  int lim = a.lens[ok ? r : 0];
+  const int most = a.limits ? a.limits[i] : cap;
+  lim = most < lim ? most : lim;
+  lim = lim < cap ? lim : cap;
+  *row = ok ? r : -1;
+  return ok && lim > 0 ? lim : 0;
 }
 
 // the first named row that holds the whole prefix (rows[0] where none does), by one wave
@@ -372,10 +373,27 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArg
   constexpr int BYTES = V_TILES > JOIN ? (V_TILES > COLS ? V_TILES : COLS) : (JOIN > COLS ? JOIN : COLS);
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   __shared__ int ids[NID];
-  const int lane = threadIdx.x & 63, n_pre = a.hkv * a.mt * a.sp;
+  const int lane = threadIdx.x & 63, pairs = a.hkv * a.sp, n_pre = pairs * a.mt, n_own = gridDim.x - n_pre;
+  // Groups of 8 workgroups (one an XCD) of the prefix and of the rows' own tokens take turns, in proportion: the ones are bound by the matrix cores
+  // where there are many columns, the others by memory, and they share the CUs. What is left of either after its last whole group comes at the end.
+  int x = blockIdx.x, p_at = -1;   // p_at: index among the prefix's items; x: among the others
+  {
+    const int gp = n_pre >> 3, gall = gp + (n_own >> 3), g8 = x >> 3, l8 = x & 7;
+    if (g8 < gall) {
+      const int before = (int)((long)g8 * gp / gall), after = (int)((long)(g8 + 1) * gp / gall);
+      if (after > before) p_at = before * 8 + l8;
+      else x = (g8 - before) * 8 + l8;
+    } else {
+      x -= gall * 8;
+      if (x < (n_pre & 7)) p_at = gp * 8 + x;
+      else x = (n_own >> 3) * 8 + x - (n_pre & 7);
+    }
+  }
   Item it;
-  if ((int)blockIdx.x < n_pre) {
-    const int pairs = a.hkv * a.sp, pair = blockIdx.x % pairs, mt = blockIdx.x / pairs;   // column tiles of one key range: one XCD where pairs % 8 == 0
+  if (p_at >= 0) {
+    int pair, mt;   // the column tiles of one key range behind one another and, where pairs divide by 8, on one XCD
+    if ((pairs & 7) == 0) { pair = (p_at / 8 / a.mt) * 8 + (p_at & 7); mt = p_at / 8 % a.mt; }
+    else { pair = p_at / a.mt; mt = p_at % a.mt; }
     it.kvh = pair % a.hkv;
     it.part = pair / a.hkv;
     const int per = ((a.prefix + KT - 1) / KT + a.sp - 1) / a.sp * KT;
@@ -389,7 +407,6 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArg
     else keys_item<T, HD, QT>(a, it, smem, ids);
     return;
   }
-  int x = blockIdx.x - n_pre;
   it.kvh = x % a.hkv; x /= a.hkv;
   const int gt = x % a.gt; x /= a.gt;
   const int sx = x % a.ss, i = x / a.ss;
@@ -412,34 +429,50 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArg
   keys_item<T, HD, 1>(a, it, smem, ids);
 }
 
-// one wave per (query, head): lane s holds part s
+// One wave per (query, head): lane s holds the weight of part s; then the lanes hold the head's dims, 16 bytes each, and a wave reads 64 * 4 / HD
+// parts at a time, the loads of four such groups in flight.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
-  const int lane = threadIdx.x & 63;
+  constexpr int LD = HD / 4, G = 64 / LD;     // lanes of a part, parts a wave reads at once
+  const int lane = threadIdx.x & 63, sub = lane / LD, d = lane % LD * 4;
   const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (id >= (long)a.n * a.hq) return;
   const int parts = a.sp + a.ss;
   float m = -INFINITY, l = 0.f;
   if (lane < parts) { m = a.ml[2 * (id * parts + lane)]; l = a.ml[2 * (id * parts + lane) + 1]; }
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float* po = a.po + id * parts * HD + d;
+  f32x4 v[4];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * G + sub;
+      v[u] = *(const f32x4*)(po + (size_t)(s < parts ? s : parts - 1) * HD);
+    }
+  };
+  load(0);
   if (l == 0.f) m = -INFINITY;
   const float mx = wave_max(m);
   const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f((m - mx) * a.c);
   const float sum = wave_sum(l * f);
-  float acc[HD / 64];
+  for (int s0 = 0; s0 < parts; s0 += 4 * G) {
+    if (s0) load(s0);
 #pragma unroll
-  for (int d = 0; d < HD / 64; ++d) acc[d] = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    if (__shfl(l, s, 64) == 0.f) continue;
-    const float fs = __shfl(f, s, 64);
-    const float* po = a.po + (id * parts + s) * HD + lane * (HD / 64);
-#pragma unroll
-    for (int d = 0; d < HD / 64; ++d) acc[d] = fmaf(po[d], fs, acc[d]);
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * G + sub;
+      const float fs = __shfl(f, s & 63, 64), ls = __shfl(l, s & 63, 64);
+      if (s < parts && ls != 0.f) acc += v[u] * fs;   // a part without tokens was not written
+    }
   }
+#pragma unroll
+  for (int o = LD; o < 64; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
+  if (sub) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int i = (int)(id / a.hq), head = (int)(id % a.hq);
-  T* op = (T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + lane * (HD / 64);
-  if constexpr (HD == 128) *(uint32_t*)op = cvt2<T>(acc[0] * inv, acc[1] * inv);
-  else *op = (T)(acc[0] * inv);
+  u32x2 st = {cvt2<T>(acc[0] * inv, acc[1] * inv), cvt2<T>(acc[2] * inv, acc[3] * inv)};
+  *(u32x2*)((T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + d) = st;
 }
 
 // how a call is split; the same for the scratch size and the launch

@@ -45,18 +45,40 @@ __device__ int block_scan(int v, int* total, int* sh) {
   return sh[w] + inc - v;
 }
 
-// the `need` lowest free pages, ascending, to list; false where there are fewer
+// The `need` lowest free pages, ascending, to list; false where there are fewer. 16 pages a thread at a time, all their loads in flight at once;
+// it stops as soon as it has enough.
 __device__ bool lowest_free(const Pages& p, int need, int* list, int* sh) {
-  const int per = (p.n_pages + NT - 1) / NT, lo = threadIdx.x * per;
-  const int hi = lo + per < p.n_pages ? lo + per : p.n_pages;
-  int mine = 0;
-  for (int i = lo; i < hi; ++i) mine += p.refs[i] == 0;
-  int total, at = block_scan(mine, &total, sh);
-  if (total < need) return false;
-  for (int i = lo; i < hi && at < need; ++i)
-    if (p.refs[i] == 0) list[at++] = i;
+  constexpr int PER = 16;
+  int found = 0;
+  for (int base = 0; base < p.n_pages && found < need; base += NT * PER) {
+    const int lo = base + (int)threadIdx.x * PER;
+    int r[PER], mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) r[j] = p.refs[lo + j < p.n_pages ? lo + j : p.n_pages - 1];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine += lo + j < p.n_pages && r[j] == 0;
+    int total, at = found + block_scan(mine, &total, sh);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (lo + j < p.n_pages && r[j] == 0) {
+        if (at < need) list[at] = lo + j;
+        ++at;
+      }
+    found += total;
+  }
+  __threadfence_block();
   __syncthreads();
-  return true;
+  return found >= need;
+}
+
+// the last of n entries whose first[] (ascending) is at most x; entries of no size start where the next does and are passed over
+__device__ __forceinline__ int entry_of(const int* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
 }
 
 __device__ __forceinline__ int pages_of(const Pages& p, int tokens) { return (tokens + p.ps - 1) >> p.log_ps; }
@@ -88,7 +110,7 @@ __device__ int block_or(int v, int* sh) {
 __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, const int* counts, int n, int* slots, int total) {
   __shared__ int sh[NT / 64 + 1];
   __shared__ unsigned seen[2048];
-  __shared__ int tok0[NT + 1], from[NT], of[NT];   // first new token, tokens held before, row of every list entry
+  __shared__ int tok0[NT], page0[NT], from[NT], of[NT];   // of every list entry: first new token, first new page, tokens held before, row
   const int t = threadIdx.x;
   int bad = check_rows(p, rows, n, seen);
   int r = 0, old = 0, add = 0;
@@ -102,43 +124,34 @@ __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, c
   }
   bad = block_or(bad, sh);
   int need_all = 0, add_all = 0, at = 0, first = 0;
-  const int have = pages_of(p, old);
   if (!bad) {
     first = block_scan(add, &add_all, sh);
-    if (add_all > total || add_all < 0) bad = ORC_KV_BAD_COUNT;
+    if (add_all > total) bad = ORC_KV_BAD_COUNT;
   }
+  int* list = p.work + 8;
   if (!bad) {
-    at = block_scan(pages_of(p, old + add) - have, &need_all, sh);
-    if (!lowest_free(p, need_all, p.work + 8, sh)) bad = ORC_KV_POOL_FULL;
+    at = block_scan(pages_of(p, old + add) - pages_of(p, old), &need_all, sh);
+    if (need_all > p.n_pages || !lowest_free(p, need_all, list, sh)) bad = ORC_KV_POOL_FULL;
   }
   if (bad) {   // the same for all threads
     if (t == 0) atomicOr(p.status, bad);
     for (int i = t; i < total; i += NT) slots[i] = -1;
     return;
   }
-  tok0[t] = first; from[t] = old; of[t] = r;
-  if (t == 0) tok0[NT] = add_all;
-  if (t < n) {
-    const int need = pages_of(p, old + add) - have;
-    for (int j = 0; j < need; ++j) {
-      const int page = p.work[8 + at + j];
-      p.refs[page] = 1;
-      p.table[(size_t)r * p.width + have + j] = page;
-    }
-    p.lens[r] = old + add;
-  }
-  __threadfence_block();
+  tok0[t] = first; page0[t] = at; from[t] = old; of[t] = r;
   __syncthreads();
+  for (int x = t; x < need_all; x += NT) {
+    const int e = entry_of(page0, n, x), page = list[x];
+    p.refs[page] = 1;
+    p.table[(size_t)of[e] * p.width + pages_of(p, from[e]) + x - page0[e]] = page;
+  }
+  if (t < n) p.lens[r] = old + add;
   for (int i = t; i < total; i += NT) {
     int s = -1;
     if (i < add_all) {
-      int lo = 0, hi = n;   // the last entry that starts at or before token i (entries without tokens start where the next does)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tok0[mid] <= i) lo = mid; else hi = mid;
-      }
-      const int pos = from[lo] + i - tok0[lo];
-      s = p.table[(size_t)of[lo] * p.width + (pos >> p.log_ps)] * p.ps + (pos & (p.ps - 1));
+      const int e = entry_of(tok0, n, i), pos = from[e] + i - tok0[e], j = (pos >> p.log_ps) - pages_of(p, from[e]);   // j < 0: the part page
+      const int page = j < 0 ? p.table[(size_t)of[e] * p.width + (pos >> p.log_ps)] : list[page0[e] + j];
+      s = page * p.ps + (pos & (p.ps - 1));
     }
     slots[i] = s;
   }
@@ -163,7 +176,9 @@ __global__ __launch_bounds__(256) void append_kernel(Pages p, const int* slots, 
 __global__ __launch_bounds__(NT) void fork_kernel(Pages p, const int* src, const int* dst, int n, int n_tokens, int share) {
   __shared__ int sh[NT / 64 + 1];
   __shared__ unsigned seen[2048];
+  __shared__ int src_of[NT], dst_of[NT], len_of[NT], page0[NT], most_sh;   // of every pair; page0: its first fresh page
   const int t = threadIdx.x;
+  if (t == 0) most_sh = 0;
   int bad = check_rows(p, dst, n, seen);
   __syncthreads();
   int s = 0, d = 0, len = 0;
@@ -180,39 +195,47 @@ __global__ __launch_bounds__(NT) void fork_kernel(Pages p, const int* src, const
     }
   }
   const int used = pages_of(p, len), keep = share ? len >> p.log_ps : 0;
-  if (t < n && !bad)
-    for (int j = 0; j < used; ++j) {
-      const int page = p.table[(size_t)s * p.width + j];
-      if (page < 0 || page >= p.n_pages) bad = ORC_KV_BAD_PAGE;
-    }
+  atomicMax(&most_sh, used);
   bad = block_or(bad, sh);
   int need_all = 0, at = 0;
+  if (!bad) at = block_scan(used - keep, &need_all, sh);
+  src_of[t] = s; dst_of[t] = d; len_of[t] = len; page0[t] = at;
+  __syncthreads();
+  const int most = most_sh;   // the pairs' pages as a grid of n x most
   if (!bad) {
-    at = block_scan(used - keep, &need_all, sh);
-    if (need_all < 0 || need_all > p.n_pages || !lowest_free(p, need_all, p.work + 8, sh)) bad = ORC_KV_POOL_FULL;
+    int off = 0;
+    for (int x = t; x < n * most; x += NT) {
+      const int i = x / most, j = x - i * most;
+      if (j >= pages_of(p, len_of[i])) continue;
+      const int page = p.table[(size_t)src_of[i] * p.width + j];
+      if (page < 0 || page >= p.n_pages) off = ORC_KV_BAD_PAGE;
+    }
+    bad = block_or(off, sh);
   }
+  // the copies: to work[8 + c], from work[8 + n_pages + c], tokens work[8 + 2 n_pages + c]
+  int* list = p.work + 8;
+  if (!bad && (need_all > p.n_pages || !lowest_free(p, need_all, list, sh))) bad = ORC_KV_POOL_FULL;
   if (bad) {
     if (t == 0) { atomicOr(p.status, bad); p.work[W_COUNT] = 0; }
     return;
   }
-  // the copies: to work[8 + i], from work[8 + n_pages + i], tokens work[8 + 2 n_pages + i]
-  if (t < n) {
-    for (int j = 0; j < used; ++j) {
-      const int from = p.table[(size_t)s * p.width + j];
-      int to = from;
-      if (j < keep) {
-        atomicAdd(&p.refs[from], 1);
-      } else {
-        const int c = at + j - keep;
-        to = p.work[8 + c];
-        p.refs[to] = 1;
-        p.work[8 + p.n_pages + c] = from;
-        p.work[8 + 2 * p.n_pages + c] = len - j * p.ps < p.ps ? len - j * p.ps : p.ps;
-      }
-      p.table[(size_t)d * p.width + j] = to;
+  for (int x = t; x < n * most; x += NT) {
+    const int i = x / most, j = x - i * most, tokens = len_of[i];
+    if (j >= pages_of(p, tokens)) continue;
+    const int from = p.table[(size_t)src_of[i] * p.width + j], kept = share ? tokens >> p.log_ps : 0;
+    int to = from;
+    if (j < kept) {
+      atomicAdd(&p.refs[from], 1);
+    } else {
+      const int c = page0[i] + j - kept;
+      to = list[c];
+      p.refs[to] = 1;
+      list[p.n_pages + c] = from;
+      list[2 * p.n_pages + c] = tokens - j * p.ps < p.ps ? tokens - j * p.ps : p.ps;
     }
-    p.lens[d] = len;
+    p.table[(size_t)dst_of[i] * p.width + j] = to;
   }
+  if (t < n) p.lens[d] = len;
   if (t == 0) p.work[W_COUNT] = need_all;
 }
 
