@@ -1,10 +1,8 @@
 // Causal attention over whole prompts packed one behind the other (orc_attention_packed), grouped heads, bf16 / fp16.
 //
 // out[t] = sum_j p_j v_j / sum_j p_j, p_j = exp2(c (q_t . k_j - m)), c = scale * log2(e), j over the tokens 0..t of t's sequence, with the running
-// maximum m and sum of one pass over the keys (flash32.h). One workgroup = NW waves x 32 query rows of one head; K / V tiles of 64 keys
-// arrive by LDS-DMA in a 2-deep ring: wait for the tile -> barrier -> issue the next one's DMA -> compute.
+// maximum m and sum of one pass over the keys (flash32.h). One workgroup = 4 waves x 32 query rows of one head.
 #include <algorithm>
-#include <type_traits>
 
 #include "../../include/oracle_hip.h"
 #include "kernels.h"
@@ -23,13 +21,57 @@ struct PackedArgs {
   float c;   // scale * log2(e)
 };
 
+// where the tiles come from and what a wave may see of them (flash_loop)
+template <typename T, int HD> struct PackedSrc {
+  typedef Tile64<HD> Tile;
+  static constexpr int RND = Tile::KEYS * Tile::CH / 256;    // DMA instructions per wave and image
+  static constexpr int KPR = 256 / Tile::CH;                 // keys one round of them covers
+  static_assert(KPR % 16 == 0, "the swizzle repeats every 16 keys: the rounds share it");
+  const T *kb, *vb;
+  long k_ts, v_ts;
+  int len, qrow, w, h;
+  int koff, voff;                        // bytes, of the lane in round 0
+  __amdgpu_buffer_rsrc_t kr, vr;         // of the tile that is asked for next
+  // Lane p of round r fills chunk p % CH of key r KPR + p / CH.
+  __device__ __forceinline__ void init(int tid) {
+    const int key_p = tid / Tile::CH;
+    w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    h = (tid & 63) >> 5;
+    koff = (int)(key_p * k_ts + Tile::swz_k(key_p, tid % Tile::CH) * 8) * 2;
+    voff = (int)(key_p * v_ts + Tile::swz_v(key_p, tid % Tile::CH) * 8) * 2;
+  }
+  // Buffer descriptors that start at the tile and end with the sequence: what lies behind the last token arrives as zeros, without a test. (The whole
+  // offset is in the lane's: a scalar one beyond the end would wrap the range check.)
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(const T* base, long ts, int t) const {
+    int left = len - t * Tile::KEYS;
+    left = left < Tile::KEYS ? left : Tile::KEYS;
+    const int bytes = (int)((left - 1) * ts + HD) * 2;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long)t * Tile::KEYS * ts), 0, left > 0 ? bytes : 0, 0x00020000);
+  }
+  __device__ __forceinline__ void next(int t) {
+    kr = tile(kb, k_ts, t + 2);
+    vr = tile(vb, v_ts, t + 1);
+  }
+  __device__ __forceinline__ void K(int, int r, char* to) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void_t*)(to + w * 1024 + r * 4096), 16, koff + (int)(r * KPR * k_ts * 2), 0, 0, 0);
+  }
+  __device__ __forceinline__ void V(int, int r, char* to) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void_t*)(to + w * 1024 + r * 4096), 16, voff + (int)(r * KPR * v_ts * 2), 0, 0, 0);
+  }
+  // Only a wave's last tile has keys in a query's future: tiles are 64 keys, the wave's queries 32 from a multiple of 32 on.
+  __device__ __forceinline__ void mask_last(int t, f32x16 (&s)[2]) const {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (t * Tile::KEYS + Flash32<T, HD>::key_of(b, i, h) > qrow) s[b][i] = -INFINITY;
+  }
+};
+
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void packed_kernel(PackedArgs a) {
   typedef Tile64<HD> Tile;
-  constexpr int KB = 64, NT = 256;
-  constexpr int RND = KB * Tile::CH / NT;    // DMA instructions per wave, operand and tile
-  constexpr int KPR = NT / Tile::CH;         // keys one round of them covers
-  __shared__ __attribute__((aligned(16))) char smem[4 * Tile::BYTES];   // K of even and odd tiles, V of even and odd tiles
+  __shared__ __attribute__((aligned(16))) char k0[Tile::BYTES], k1[Tile::BYTES], v0[Tile::BYTES], v1[Tile::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   // Workgroup ids go round robin over the 8 XCDs: where the heads divide by 8 an XCD keeps hq / 8 of them, so the tiles that read the
   // same K / V run on one L2. The plan lists long tiles first.
@@ -49,104 +91,18 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(PackedArgs a) {
   const int seq = wk.x, len = wk.y, q0 = wk.z;
   if (seq < 0 || q0 < 0 || len <= q0 || len > a.total - seq) return;   // a plan of other prompts than these
   const int kvh = head / a.group;
-  const T* kb = (const T*)a.k + (size_t)seq * a.k_ts + (size_t)kvh * a.k_hs;
-  const T* vb = (const T*)a.v + (size_t)seq * a.v_ts + (size_t)kvh * a.v_hs;
+  PackedSrc<T, HD> src;
+  src.kb = (const T*)a.k + (size_t)seq * a.k_ts + (size_t)kvh * a.k_hs;
+  src.vb = (const T*)a.v + (size_t)seq * a.v_ts + (size_t)kvh * a.v_hs;
+  src.k_ts = a.k_ts; src.v_ts = a.v_ts; src.len = len;
   const int qw = q0 + w * 32, qrow = qw + (lane & 31);
+  src.qrow = qrow;
+  src.init(tid);
   Flash32<T, HD> f;
   f.init((const T*)a.q + (size_t)(seq + (qrow < len ? qrow : len - 1)) * a.q_ts + (size_t)head * a.q_hs, lane);
   const int k_end = q0 + ROWS < len ? q0 + ROWS : len;
-
-  // Lane p of round r fills chunk p % CH of key r KPR + p / CH. The swizzle looks at the key's low bits only, which the rounds share.
-  const int key_p = tid / Tile::CH, ch_p = tid % Tile::CH;
-  const int ck = Tile::swz_k(key_p, ch_p) * 8, cv = Tile::swz_v(key_p, ch_p) * 8;
-  static_assert(KPR % 16 == 0, "the swizzle repeats every 16 keys");
-  const unsigned koff = (unsigned)(key_p * a.k_ts + ck), voff = (unsigned)(key_p * a.v_ts + cv);
-  auto dma = [&](const T* base, long ts, unsigned off, int c, int k0, char* to) {
-    to += w * 1024;
-    if (k0 + KB <= len) {
-      const T* from = base + (size_t)k0 * ts;
-#pragma unroll
-      for (int r = 0; r < RND; ++r)
-        __builtin_amdgcn_global_load_lds((glb_void_t*)(from + (size_t)r * KPR * ts + off), (lds_void_t*)(to + r * NT * 16), 16, 0, 0);
-    } else {
-#pragma unroll
-      for (int r = 0; r < RND; ++r) {
-        int src = k0 + r * KPR + key_p;
-        src = src < len ? src : len - 1;   // behind the last token: that token again, its score is masked
-        __builtin_amdgcn_global_load_lds((glb_void_t*)(base + (size_t)src * ts + c), (lds_void_t*)(to + r * NT * 16), 16, 0, 0);
-      }
-    }
-  };
-  auto dma_k = [&](int k0, int stage) { dma(kb, a.k_ts, koff, ck, k0, smem + stage * Tile::BYTES); };
-  auto dma_v = [&](int k0, int stage) { dma(vb, a.v_ts, voff, cv, k0, smem + (2 + stage) * Tile::BYTES); };
-  // One iteration a tile t: wait for its values and the next tile's keys, barrier (the waves are through with the tile before), ask for what comes
-  // behind those. PAR = t % 2.
-  const int tiles = (k_end + KB - 1) / KB;
-  auto advance = [&](int t, auto par) {
-    constexpr int PAR = decltype(par)::value;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 2 < tiles) dma_k((t + 2) * KB, PAR);
-    if (t + 1 < tiles) dma_v((t + 1) * KB, PAR ^ 1);
-  };
-  float tm = 0.f;
-  // tile t, whose scores are in s: the next tile's scores (to n) between this one's exponentials, then this one's values
-  auto step = [&](int t, const f32x16 (&s)[2], f32x16 (&n)[2], auto par) {
-    constexpr int PAR = decltype(par)::value;
-    advance(t, par);
-    f.raise(tm, a.c);
-    const float mc = f.base(a.c);
-    const char* sK = smem + (PAR ^ 1) * Tile::BYTES;
-    u32x4 pf[4];
-    n[0] = f.scores(sK, 0);
-    f.weights(s[0], a.c, mc, pf);
-    n[1] = f.scores(sK, 1);
-    f.weights(s[1], a.c, mc, pf + 2);
-    f.values(smem + (2 + PAR) * Tile::BYTES, pf);
-    tm = f.largest(n);
-  };
-  // the wave's last tile, the only one with keys in a query's future: tiles are 64 keys, the wave's queries 32 from a multiple of 32 on
-  auto finish = [&](int t, f32x16 (&s)[2], auto par) {
-    constexpr int PAR = decltype(par)::value;
-    advance(t, par);
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (t * KB + Flash32<T, HD>::key_of(b, i, h) > qrow) s[b][i] = -INFINITY;
-    f.add(smem + (2 + PAR) * Tile::BYTES, s, a.c);
-  };
-  typedef std::integral_constant<int, 0> even;
-  typedef std::integral_constant<int, 1> odd;
-  dma_k(0, 0);
-  dma_v(0, 0);
-  if (tiles > 1) {
-    dma_k(KB, 1);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * RND) : "memory");
-  } else {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RND) : "memory");
-  }
-  __syncthreads();
-  const int mine = qw >= len ? 0 : (qw + 31) / KB + 1;   // the wave's tiles: those behind are all in its future; 0: it has no query
-  int t = 0;
-  if (mine) {
-    f32x16 s[2] = {f.scores(smem, 0), f.scores(smem, 1)}, n[2];
-    tm = f.largest(s);
-    for (; t + 2 < mine; t += 2) {
-      step(t, s, n, even());
-      step(t + 1, n, s, odd());
-    }
-    if (t + 1 < mine) {
-      step(t, s, n, even());
-      finish(t + 1, n, odd());
-    } else {
-      finish(t, s, even());
-    }
-  }
-  for (t = mine; t < tiles; ++t) {   // the other waves' tiles
-    if (t & 1) advance(t, odd());
-    else advance(t, even());
-  }
+  // the wave's tiles: those behind are all in its future; 0: it has no query
+  flash_loop(f, src, Images{k0, k1, v0, v1}, (k_end + Tile::KEYS - 1) / Tile::KEYS, qw >= len ? 0 : (qw + 31) / Tile::KEYS + 1, a.c);
   const float inv = 1.0f / f.total();
   if (qrow >= len) return;
   T* op = (T*)a.o + (size_t)(seq + qrow) * a.o_ts + (size_t)head * a.o_hs;

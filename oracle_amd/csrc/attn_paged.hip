@@ -21,7 +21,8 @@
 namespace {
 
 constexpr int KT = 32;            // keys of a wave's tile in keys_item
-constexpr int NID = 512;          // page ids held in LDS at a time
+constexpr int IDS = 512;          // page ids held in LDS at a time by keys_item
+constexpr int IDS_COLS = 2048;    // by cols_item, whose range has to fit
 constexpr int MAX_PARTS = 64;     // parts of one query (a lane of the combining wave each)
 
 struct AttendArgs {
@@ -72,14 +73,17 @@ __device__ __forceinline__ int prefix_row(const AttendArgs& a, int lane) {
 // What a workgroup does: the keys [k_lo, k_hi) of row `row` for `cols` query columns of K/V head kvh, from column f0 (query, head of the group) on
 struct Item { int kvh, part, k_lo, k_hi, row, f0, cols; };
 
-// ids[e] = page of the tokens [(first + e) ps, ...) of the row, -1 outside the pool; by the whole workgroup
-__device__ __forceinline__ void load_ids(const AttendArgs& a, int row, int first, int count, int* ids) {
+// ids[e] = page of the tokens [(first + e) ps, ...) of the row, -1 outside the pool; by the whole workgroup. Returns whether any is outside,
+// or `odd` is set in any thread.
+__device__ __forceinline__ bool load_ids(const AttendArgs& a, int row, int first, int count, int* ids, bool odd = false) {
   __syncthreads();
   for (int e = threadIdx.x; e < count; e += 256) {
-    const int p = row < 0 ? -1 : a.table[(size_t)row * a.width + first + e];
-    ids[e] = p < a.n_pages ? p : -1;
+    int p = row < 0 ? -1 : a.table[(size_t)row * a.width + first + e];
+    p = p < a.n_pages ? p : -1;
+    ids[e] = p;
+    odd |= p < 0;
   }
-  __syncthreads();
+  return __syncthreads_or(odd);
 }
 
 // One part of one column's result: m, sum and the output sums of dims d..d+3 (want_ml: by the caller that holds d == 0); the result itself where the
@@ -99,8 +103,12 @@ __device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col
   }
 }
 
-template <typename T, int HD, int QT>
-__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, char* smem, int* ids) {
+// LDS of keys_item: a V tile for each wave and, behind the loop, the waves' maxima, sums and outputs, in the same four rooms. step: their distance in
+// one array (picking a room by address arithmetic takes fewer registers, and 128 are the limit), 0 where they are arrays of their own.
+struct Rooms { char* r[4]; int step; };
+
+template <typename T, int HD, int QT, int NID>
+__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids) {
   typedef typename Mma<T>::v8 v8;
   constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH, MT = 16 * QT;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
@@ -128,7 +136,7 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
   }
   const T* kb = (const T*)a.k + (size_t)it.kvh * ps * HD + g * 8;
   const T* vb = (const T*)a.v + (size_t)it.kvh * ps * HD;
-  char* sV = smem + w * TILE;
+  char* sV = room.step ? room.r[0] + w * room.step : w == 0 ? room.r[0] : w == 1 ? room.r[1] : w == 2 ? room.r[2] : room.r[3];
   const int key_p = lane / CH, ch_p = lane % CH;
   for (int kc = it.k_lo; kc < it.k_hi; kc += (NID - 2) << a.log_ps) {
     const int first = kc >> a.log_ps, ke = kc + ((NID - 2) << a.log_ps) < it.k_hi ? kc + ((NID - 2) << a.log_ps) : it.k_hi;
@@ -215,8 +223,8 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
 
   // join the four waves: maxima and sums of all, then the outputs of waves 2, 3 into 0, 1 and of 1 into 0
   __syncthreads();
-  float* sm = (float*)smem;                  // [4][MT] maxima, [4][MT] sums, then [2][MT][HD]
-  float* so = sm + 8 * MT;
+  float* sm = (float*)room.r[0];             // [4][MT] maxima, [4][MT] sums
+  float* so = (float*)(w & 1 ? room.r[2] : room.r[1]);   // [MT][HD] of a pair of waves
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
@@ -243,17 +251,18 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
 #pragma unroll
   for (int half = 2; half >= 1; half >>= 1) {
     if (w >= half && w < 2 * half) {
+      float* to = half == 2 ? so : (float*)room.r[1];   // wave 3 to 1, 2 to 0; then 1 to 0
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) *(f32x4*)(so + (size_t)((w - half) * MT + t * 16 + c16) * HD + d * 16 + 4 * g) = o[t][d];
+        for (int d = 0; d < HD / 16; ++d) *(f32x4*)(to + (size_t)(t * 16 + c16) * HD + d * 16 + 4 * g) = o[t][d];
     }
     __syncthreads();
     if (w < half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[t][d] += *(const f32x4*)(so + (size_t)(w * MT + t * 16 + c16) * HD + d * 16 + 4 * g);
+        for (int d = 0; d < HD / 16; ++d) o[t][d] += *(const f32x4*)(so + (size_t)(t * 16 + c16) * HD + d * 16 + 4 * g);
     }
     __syncthreads();
   }
@@ -266,145 +275,127 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
   }
 }
 
-template <typename T, int HD>
-__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, char* smem, int* ids) {
+// Where cols_item's tiles come from (flash_loop): the pages ids[] of the tokens [kc, ke), all of them in the pool. A lane holds where page win + lane
+// starts, so that an address takes two v_readlanes and no LDS round trip; the window moves on once in a while.
+template <typename T, int HD> struct PageSrc {
   typedef Tile64<HD> Tile;
-  constexpr int KB = 64, RND = KB * Tile::CH / 256, KPR = 256 / Tile::CH;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  static constexpr int RND = Tile::KEYS * Tile::CH / 256, KPR = 256 / Tile::CH, GK = KPR / 4;   // GK: keys of one DMA instruction, all on one page
+  const char *kb, *vb;
+  const int* ids;
+  unsigned page_bytes;
+  int kc, ke, first, last, log_ps, w, h, lane, win;
+  unsigned lk, lv, lo, hi;
+  __device__ __forceinline__ void window(int at) {
+    win = at;
+    const unsigned long long off = (unsigned long long)(unsigned)ids[win + lane < IDS_COLS ? win + lane : IDS_COLS - 1] * page_bytes;
+    lo = (unsigned)off;
+    hi = (unsigned)(off >> 32);
+  }
+  __device__ __forceinline__ void init(int tid) {
+    const int key_p = tid / Tile::CH;
+    w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    lane = tid & 63;
+    h = lane >> 5;
+    first = kc >> log_ps;
+    last = ((ke - 1) >> log_ps) - first;
+    lk = (unsigned)((key_p - w * GK) * HD + Tile::swz_k(key_p, tid % Tile::CH) * 8) * 2;
+    lv = (unsigned)((key_p - w * GK) * HD + Tile::swz_v(key_p, tid % Tile::CH) * 8) * 2;
+    window(0);
+  }
+  __device__ __forceinline__ void next(int t) {   // K of tile t + 2 and V of t + 1 are to come: their pages are in the window
+    const int k = (kc + (t + 3) * Tile::KEYS - 1) >> log_ps, v = (kc + (t + 1) * Tile::KEYS) >> log_ps;
+    if (min(k - first, last) - win >= 64) window(min(v - first, last));
+  }
+  // The r-th DMA instruction of tile t. A tile that begins or reaches behind the last token takes tokens of the last page instead: their
+  // scores are masked, or the tile is not read.
+  __device__ __forceinline__ void ask(const char* base, unsigned l, int t, int r, char* to) const {
+    const int k = kc + t * Tile::KEYS + r * KPR + w * GK, e = min((k >> log_ps) - first, last) - win;
+    const unsigned long long off = (unsigned)__builtin_amdgcn_readlane((int)lo, e) | (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, e) << 32;
+    const char* from = base + off + (unsigned)(k & ((1 << log_ps) - 1)) * (HD * 2);
+    __builtin_amdgcn_global_load_lds((glb_void_t*)(from + l), (lds_void_t*)(to + w * 1024 + r * 4096), 16, 0, 0);
+  }
+  __device__ __forceinline__ void K(int t, int r, char* to) const { ask(kb, lk, t, r, to); }
+  __device__ __forceinline__ void V(int t, int r, char* to) const { ask(vb, lv, t, r, to); }
+  __device__ __forceinline__ void mask_last(int t, f32x16 (&s)[2]) const {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (kc + t * Tile::KEYS + Flash32<T, HD>::key_of(b, i, h) >= ke) s[b][i] = -INFINITY;
+  }
+};
+
+template <typename T, int HD>
+__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, const Images& im, int* ids) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int ps = 1 << a.log_ps, col = w * 32 + (lane & 31);
-  const bool mine = w * 32 < it.cols;          // the wave has columns
-  Flash32<T, HD> f;
-  int lim = it.k_hi;
-  {
-    const int fc = it.f0 + (col < it.cols ? col : 0), i = fc / a.group;
-    f.init((const T*)a.q + (size_t)i * a.q_ts + (size_t)(it.kvh * a.group + fc % a.group) * a.q_hs, lane);
-    int r;
-    const int v = visible(a, i, &r);
-    if (col < it.cols && v < lim) lim = v;
-  }
-  int lim_min = lim;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const int y = __shfl_xor(lim_min, x, 64);
-    lim_min = y < lim_min ? y : lim_min;
-  }
-  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-  const T* kb = (const T*)a.k + (size_t)it.kvh * ps * HD;
-  const T* vb = (const T*)a.v + (size_t)it.kvh * ps * HD;
-  const int key_p = tid / Tile::CH, ch_p = tid % Tile::CH;
-  const int ck = Tile::swz_k(key_p, ch_p) * 8, cv = Tile::swz_v(key_p, ch_p) * 8;
-  for (int kc = it.k_lo; kc < it.k_hi; kc += (NID - 4) << a.log_ps) {
-    const int first = kc >> a.log_ps, ke = kc + ((NID - 4) << a.log_ps) < it.k_hi ? kc + ((NID - 4) << a.log_ps) : it.k_hi;
-    load_ids(a, it.row, first, ((ke - 1) >> a.log_ps) - first + 1, ids);
-    // pages of the tile's four units of 16 keys (-1: behind the end, or outside the pool); the first of those that are there, -1 without any
-    int pg[4];
-    auto units = [&](int k0) {
-      int good = -1;
-#pragma unroll
-      for (int u = 3; u >= 0; --u) {
-        pg[u] = k0 + 16 * u < ke ? __builtin_amdgcn_readfirstlane(ids[((k0 + 16 * u) >> a.log_ps) - first]) : -1;
-        if (pg[u] >= 0) good = u;
-      }
-      return good;
-    };
-    auto seek = [&](int k0, int* good) {   // the next tile with a page in the pool
-      for (; k0 < ke; k0 += KB)
-        if ((*good = units(k0)) >= 0) break;
-      return k0;
-    };
-    auto dma = [&](int k0, int good, int stage) {
-      char* sk = smem + stage * 2 * Tile::BYTES + w * 1024;
-#pragma unroll
-      for (int r = 0; r < RND; ++r) {
-        const int pu = HD == 128 ? pg[r] : w >> 1 ? pg[(2 * r + 1) & 3] : pg[(2 * r) & 3];   // page of this wave's keys in this round
-        int at = k0 + r * KPR + key_p, page = pu;
-        if (at >= ke) at = ke - 1;           // behind the last token: that token again, its score is masked
-        if (pu < 0) { page = good == 0 ? pg[0] : good == 1 ? pg[1] : good == 2 ? pg[2] : pg[3]; at = k0 + 16 * good; }
-        const size_t off = (size_t)page * a.page_elems + (size_t)((at & (ps - 1)) * HD);
-        __builtin_amdgcn_global_load_lds((glb_void_t*)(kb + off + ck), (lds_void_t*)(sk + r * 4096), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((glb_void_t*)(vb + off + cv), (lds_void_t*)(sk + Tile::BYTES + r * 4096), 16, 0, 0);
-      }
-    };
-    int good;
-    int k0 = seek(kc, &good);
-    if (k0 < ke) dma(k0, good, 0);
-    auto step = [&](auto st) {
-      constexpr int stage = decltype(st)::value;
-      const int now = k0;
-      const unsigned there = (pg[0] >= 0) | (pg[1] >= 0) << 1 | (pg[2] >= 0) << 2 | (pg[3] >= 0) << 3;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      k0 = seek(k0 + KB, &good);
-      if (k0 < ke) dma(k0, good, stage ^ 1);
-      if (!mine) return;
-      const char* sK = smem + stage * 2 * Tile::BYTES;
-      f32x16 s[2] = {f.scores(sK, 0), f.scores(sK, 1)};
-      if (there != 15u || now + KB > lim_min) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = Flash32<T, HD>::key_of(b, i, h);
-            if (now + key >= lim || !(there >> (b * 2 + (i >> 3)) & 1)) s[b][i] = -INFINITY;
-          }
-      }
-      f.add(sK + Tile::BYTES, s, a.c);
-    };
-    while (k0 < ke) {
-      step(std::integral_constant<int, 0>());
-      if (k0 < ke) step(std::integral_constant<int, 1>());
+  const int fc = it.f0 + (col < it.cols ? col : 0), i = fc / a.group;
+  int r;
+  const int lim = visible(a, i, &r);
+  const bool empty = lim == 0;             // a column whose query has no tokens (a row that has ended): what it computes is not used
+  const int first = it.k_lo >> a.log_ps;
+  if (load_ids(a, it.row, first, ((it.k_hi - 1) >> a.log_ps) - first + 1, ids, lim > 0 && lim < it.k_hi)) {
+    // a page outside the pool, or a query that ends before the prefix does: 16 columns at a time, where every key has its test
+    Item sub = it;
+    for (int x = 0; x < it.cols; x += 16) {
+      sub.f0 = it.f0 + x;
+      sub.cols = it.cols - x < 16 ? it.cols - x : 16;
+      keys_item<T, HD, 1, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids);
     }
+    return;
   }
-  const float sum = f.total();
+  PageSrc<T, HD> src;
+  src.kb = a.k + (size_t)it.kvh * ps * HD * 2;
+  src.vb = a.v + (size_t)it.kvh * ps * HD * 2;
+  src.ids = ids; src.page_bytes = (unsigned)(a.page_elems * 2); src.log_ps = a.log_ps;
+  src.kc = it.k_lo; src.ke = it.k_hi;
+  src.init(threadIdx.x);
+  Flash32<T, HD> f;
+  f.init((const T*)a.q + (size_t)i * a.q_ts + (size_t)(it.kvh * a.group + fc % a.group) * a.q_hs, lane);
+  const int tiles = (it.k_hi - it.k_lo + Tile64<HD>::KEYS - 1) / Tile64<HD>::KEYS;
+  flash_loop(f, src, im, tiles, w * 32 < it.cols ? tiles : 0, a.c);   // a wave without columns helps with the loads
+  const float sum = empty ? 0.f : f.total();
   if (col < it.cols) {
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        put<T, HD>(a, it, col, dt * 32 + 2 * i + 4 * h, f.m, sum, f32x4{f.o[dt][i], f.o[dt][i + 1], f.o[dt][i + 2], f.o[dt][i + 3]});
+      for (int j = 0; j < 16; j += 4)
+        put<T, HD>(a, it, col, dt * 32 + 2 * j + 4 * h, f.m, sum, f32x4{f.o[dt][j], f.o[dt][j + 1], f.o[dt][j + 2], f.o[dt][j + 3]});
   }
 }
 
 // PRE: how the prefix is read. 1, 2: keys_item with that many blocks of 16 columns; 8: cols_item, 128 columns
 template <typename T, int HD, int PRE>
 __global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArgs a) {
-  constexpr int QT = PRE == 8 ? 1 : PRE, MT = 16 * PRE;
-  constexpr int V_TILES = 4 * KT * HD * 2, JOIN = (8 + 2 * HD) * 16 * QT * 4, COLS = PRE == 8 ? 4 * Tile64<HD>::BYTES : 0;
-  constexpr int BYTES = V_TILES > JOIN ? (V_TILES > COLS ? V_TILES : COLS) : (JOIN > COLS ? JOIN : COLS);
-  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  constexpr int QT = PRE == 8 ? 1 : PRE, MT = 16 * PRE, NID = PRE == 8 ? IDS_COLS : IDS;
+  // a room holds a V tile, or the outputs of 16 QT columns; the tile images of cols_item are larger than either
+  constexpr int V_TILE = KT * HD * 2, JOIN = MT * HD * 4, ROOM = PRE == 8 ? Tile64<HD>::BYTES : V_TILE > JOIN ? V_TILE : JOIN;
+  constexpr int ONE = PRE == 8 ? ROOM : 16;
+  __shared__ __attribute__((aligned(16))) char r0[PRE == 8 ? ROOM : 4 * ROOM], r1[ONE], r2[ONE], r3[ONE];
+  const Rooms room = PRE == 8 ? Rooms{{r0, r1, r2, r3}, 0} : Rooms{{r0, r0 + ROOM, r0 + 2 * ROOM, r0 + 3 * ROOM}, ROOM};
   __shared__ int ids[NID];
-  const int lane = threadIdx.x & 63, pairs = a.hkv * a.sp, n_pre = pairs * a.mt, n_own = gridDim.x - n_pre;
-  // Groups of 8 workgroups (one an XCD) of the prefix and of the rows' own tokens take turns, in proportion: the ones are bound by the matrix cores
-  // where there are many columns, the others by memory, and they share the CUs. What is left of either after its last whole group comes at the end.
-  int x = blockIdx.x, p_at = -1;   // p_at: index among the prefix's items; x: among the others
-  {
-    const int gp = n_pre >> 3, gall = gp + (n_own >> 3), g8 = x >> 3, l8 = x & 7;
-    if (g8 < gall) {
-      const int before = (int)((long)g8 * gp / gall), after = (int)((long)(g8 + 1) * gp / gall);
-      if (after > before) p_at = before * 8 + l8;
-      else x = (g8 - before) * 8 + l8;
-    } else {
-      x -= gall * 8;
-      if (x < (n_pre & 7)) p_at = gp * 8 + x;
-      else x = (n_own >> 3) * 8 + x - (n_pre & 7);
-    }
-  }
+  // The prefix's items come first, the rows' own tokens behind them. (Taking turns in groups of 8 was slower, by up to 2x: workgroups are dealt round
+  // robin to an XCD's shader engines, so a regular pattern of long and short ones loads some engines with the long ones.)
+  const int lane = threadIdx.x & 63, pairs = a.hkv * a.sp, n_pre = pairs * a.mt;
+  int x = (int)blockIdx.x - n_pre;
   Item it;
-  if (p_at >= 0) {
+  if (x < 0) {
+    const int p_at = blockIdx.x;
     int pair, mt;   // the column tiles of one key range behind one another and, where pairs divide by 8, on one XCD
     if ((pairs & 7) == 0) { pair = (p_at / 8 / a.mt) * 8 + (p_at & 7); mt = p_at / 8 % a.mt; }
     else { pair = p_at / a.mt; mt = p_at % a.mt; }
     it.kvh = pair % a.hkv;
     it.part = pair / a.hkv;
-    const int per = ((a.prefix + KT - 1) / KT + a.sp - 1) / a.sp * KT;
+    constexpr int UNIT = PRE == 8 ? Tile64<HD>::KEYS : KT;
+    const int per = ((a.prefix + UNIT - 1) / UNIT + a.sp - 1) / a.sp * UNIT;
     it.k_lo = it.part * per;
     it.k_hi = it.k_lo + per < a.prefix ? it.k_lo + per : a.prefix;
     it.row = prefix_row(a, lane);
     it.f0 = mt * MT;
     it.cols = a.n * a.group - it.f0;
     if (it.cols > MT) it.cols = MT;
-    if constexpr (PRE == 8) cols_item<T, HD>(a, it, smem, ids);
-    else keys_item<T, HD, QT>(a, it, smem, ids);
+    if constexpr (PRE == 8) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids);
+    else keys_item<T, HD, QT, NID>(a, it, room, ids);
     return;
   }
   it.kvh = x % a.hkv; x /= a.hkv;
@@ -426,7 +417,7 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArg
   it.f0 = i * a.group + gt * 16;
   it.cols = a.group - gt * 16;
   if (it.cols > 16) it.cols = 16;
-  keys_item<T, HD, 1>(a, it, smem, ids);
+  keys_item<T, HD, 1, NID>(a, it, room, ids);
 }
 
 // One wave per (query, head): lane s holds the weight of part s; then the lanes hold the head's dims, 16 bytes each, and a wave reads 64 * 4 / HD
@@ -481,16 +472,21 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   Split s;
   const int group = n_heads / c->n_kv_heads;
   const int64_t cols = (int64_t)n * group;
-  s.pre = cols <= 16 ? 1 : cols <= 32 ? 2 : 8;
+  // cols_item reads at most IDS_COLS - 4 pages, 40 parts at the most
+  const int64_t range = (int64_t)(IDS_COLS - 4) * c->page_size, least_sp = (prefix + range - 1) / range;
+  s.pre = cols <= 16 ? 1 : cols <= 32 || least_sp > 40 ? 2 : 8;
   s.mt = prefix ? (int)((cols + 16 * s.pre - 1) / (16 * s.pre)) : 0;
   s.gt = (group + 15) / 16;
   s.sp = 0;
   if (prefix) {
     const int64_t base = (int64_t)c->n_kv_heads * s.mt;
-    int64_t sp = 512 / base;
+    // cols_item runs two to a CU: 384 items leave every fourth place to the rows' own tokens, which are bound by memory (96 rows, 4 heads a
+    // K/V head, 32k + 570 tokens: 264 items 131 us, 384 136, 504 143; without own tokens 96, 86, 87). keys_item: 512, of 256 keys and more.
+    int64_t sp = ((s.pre == 8 ? 384 : 512) + base - 1) / base;
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
-    s.sp = (int)(sp < 1 ? 1 : sp > 32 ? 32 : sp);
+    sp = sp < 1 ? 1 : sp > 40 ? 40 : sp;
+    s.sp = (int)(s.pre == 8 && sp < least_sp ? least_sp : sp);
   }
   const int64_t own = (int64_t)n * c->n_kv_heads * s.gt;
   const int64_t left = (int64_t)c->max_row_pages * c->page_size - prefix;
@@ -506,6 +502,7 @@ const char* bad_call(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   if (c->n_kv_heads < 1 || n_heads < 1 || n_heads % c->n_kv_heads) return "n_heads is not a multiple of n_kv_heads";
   if (n < 0 || n > 1024) return "0..1024 queries a call";
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return "page_size is 16, 32, 64 or 128";
+  if ((int64_t)c->n_kv_heads * c->page_size * 128 * 2 > 0x7fffffff) return "a page of 2 GiB and more";
   if (c->max_rows < 1 || c->n_pages < 1 || c->max_row_pages < 1 || c->max_row_pages > 1 << 20) return "bad geometry";
   if (prefix < 0 || prefix % c->page_size || (int64_t)prefix > (int64_t)c->max_row_pages * c->page_size)
     return "prefix_tokens is not a multiple of page_size inside a row";

@@ -10,6 +10,8 @@
 // more than 8 / c: p then stays below 2^8, whose rounding to 16 bits is as exact relatively as below 1, and the 64 multiplies of a
 // rescale are spent on few tiles.
 #pragma once
+#include <type_traits>
+
 #include "mma16.h"
 
 // A tile image: 64 rows (keys) of HD values, 16-byte chunk ch of a row at place swz(key, ch), an involution. The 8 lanes of a ds_read_b128 phase
@@ -47,12 +49,19 @@ template <typename T, int HD> struct Flash32 {
   }
   // scores of keys 32 b .. 32 b + 31 of a tile
   __device__ __forceinline__ f32x16 scores(const char* sK, int b) const {
+    f32x16 s = zero();
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) s = score(sK, b, kk, s);
+    return s;
+  }
+  static __device__ __forceinline__ f32x16 zero() {
     f32x16 s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk) s = Mma<T>::m32(*(const v8*)(sK + ka[kk] + b * 32 * Tile::ROWB), qf[kk], s);
     return s;
+  }
+  __device__ __forceinline__ f32x16 score(const char* sK, int b, int kk, f32x16 s) const {
+    return Mma<T>::m32(*(const v8*)(sK + ka[kk] + b * 32 * Tile::ROWB), qf[kk], s);
   }
   // key of s[b][i] inside the tile
   static __device__ __forceinline__ int key_of(int b, int i, int h) { return b * 32 + 8 * (i >> 2) + 4 * h + (i & 3); }
@@ -106,3 +115,99 @@ template <typename T, int HD> struct Flash32 {
   }
   __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
+
+// The LDS images of even and odd tiles. Four arrays of their own, not one: the compiler then sees that a transposing read of one does not touch what the
+// DMA in flight writes, and does not wait for that DMA in front of it.
+struct Images { char *k0, *k1, *v0, *v1; };
+
+// The loop over the tiles of a workgroup of 4 waves, keys asked for two tiles ahead and values one. Iteration t waits for its values and the next
+// tile's keys, then a barrier (the waves are through with tile t - 1). The products of tile t + 1's scores stand between the exponentials of
+// tile t, so the matrix cores work through the softmax, and the DMA instructions stand between the products: issued in one go they held the
+// wave up for 1300 of 3700 cycles an iteration (the path to L1 takes 64 bytes a cycle, a tile is 32 KiB).
+// All waves make all `tiles` iterations, a wave computes in the first `mine` of them. src supplies
+//   RND                  DMA instructions a wave issues for an image
+//   K(t, r, to), V(...)  the r-th of them for a tile; t >= tiles: any tile, it is not read
+//   mask_last(t, s)      sets the scores of keys that are not to be seen to -inf in the wave's last tile; in the others all are seen
+// (A mask or a test inside the steps would cost registers the pipeline does not have: 256 are in use at head dim 128.)
+template <typename T, int HD, typename Src>
+__device__ __forceinline__ void flash_loop(Flash32<T, HD>& f, Src& src, const Images& im, int tiles, int mine, float c) {
+  typedef std::integral_constant<int, 0> even;
+  typedef std::integral_constant<int, 1> odd;
+  constexpr int RND = Src::RND, NK = HD / 16, EVERY = NK / RND;
+  auto arrive = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  auto fetch = [&](int t, auto par) {   // what iteration t asks for
+    constexpr int PAR = decltype(par)::value;
+#pragma unroll
+    for (int r = 0; r < RND; ++r) src.K(t + 2, r, PAR ? im.k1 : im.k0);
+#pragma unroll
+    for (int r = 0; r < RND; ++r) src.V(t + 1, r, PAR ? im.v0 : im.v1);
+  };
+  float tm = 0.f;
+  // tile t, whose scores are in s; the next tile's go to n
+  auto step = [&](int t, const f32x16 (&s)[2], f32x16 (&n)[2], auto par) {
+    constexpr int PAR = decltype(par)::value;
+    arrive();
+    f.raise(tm, c);
+    const float mc = f.base(c);
+    const char* sK = PAR ? im.k0 : im.k1;
+    u32x4 pf[4];
+    src.next(t);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      n[b] = f.zero();
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        n[b] = f.score(sK, b, kk, n[b]);
+        if (kk % EVERY == EVERY - 1) {
+          if (b == 0) src.K(t + 2, kk / EVERY, PAR ? im.k1 : im.k0);
+          else src.V(t + 1, kk / EVERY, PAR ? im.v0 : im.v1);
+        }
+      }
+      f.weights(s[b], c, mc, pf + 2 * b);
+    }
+    f.values(PAR ? im.v1 : im.v0, pf);
+    tm = f.largest(n);
+  };
+  auto finish = [&](int t, f32x16 (&s)[2], auto par) {
+    constexpr int PAR = decltype(par)::value;
+    arrive();
+    src.next(t);
+    fetch(t, par);
+    src.mask_last(t, s);
+    f.add(PAR ? im.v1 : im.v0, s, c);
+  };
+  src.next(-2);
+#pragma unroll
+  for (int r = 0; r < RND; ++r) src.K(0, r, im.k0);
+  src.next(-1);
+#pragma unroll
+  for (int r = 0; r < RND; ++r) src.V(0, r, im.v0);
+#pragma unroll
+  for (int r = 0; r < RND; ++r) src.K(1, r, im.k1);
+  arrive();
+  int t = 0;
+  if (mine > 0) {
+    f32x16 s[2] = {f.scores(im.k0, 0), f.scores(im.k0, 1)}, n[2];
+    tm = f.largest(s);
+    for (; t + 2 < mine; t += 2) {
+      step(t, s, n, even());
+      step(t + 1, n, s, odd());
+    }
+    if (t + 1 < mine) {
+      step(t, s, n, even());
+      finish(t + 1, n, odd());
+    } else {
+      finish(t, s, even());
+    }
+  }
+  for (t = mine; t < tiles; ++t) {   // the other waves' tiles
+    arrive();
+    src.next(t);
+    if (t & 1) fetch(t, odd());
+    else fetch(t, even());
+  }
+  arrive();   // what was asked for behind the last tile
+}

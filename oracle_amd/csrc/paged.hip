@@ -350,6 +350,7 @@ const char* bad_cache(const orc_kv_pages* c) {
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return "page_size is 16, 32, 64 or 128";
   if (c->head_dim != 64 && c->head_dim != 128) return "head_dim is 64 or 128";
   if (c->dtype != 0 && c->dtype != 1) return "dtype is 0 (bf16) or 1 (fp16)";
+  if ((int64_t)c->n_kv_heads * c->page_size * c->head_dim * 2 > 0x7fffffff) return "a page of 2 GiB and more";
   if ((int64_t)c->n_pages * c->page_size > 0x7fffffff) return "more than 2^31 - 1 tokens in the pool";
   if (c->max_row_pages > 1 << 20) return "more than 2^20 pages a row";   // 1024 rows' pages add up in 32 bits
   if ((uintptr_t)c->kv & 15) return "kv is not aligned to 16 bytes";
