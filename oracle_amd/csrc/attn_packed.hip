@@ -69,7 +69,7 @@ template <typename T, int HD> struct PackedSrc {
 };
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, 2) void packed_kernel(PackedArgs a) {
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_kernel(PackedArgs a) {
   typedef Tile64<HD> Tile;
   __shared__ __attribute__((aligned(16))) char k0[Tile::BYTES], k1[Tile::BYTES], v0[Tile::BYTES], v1[Tile::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -102,17 +102,12 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(PackedArgs a) {
   f.init((const T*)a.q + (size_t)(seq + (qrow < len ? qrow : len - 1)) * a.q_ts + (size_t)head * a.q_hs, lane);
   const int k_end = q0 + ROWS < len ? q0 + ROWS : len;
   // the wave's tiles: those behind are all in its future; 0: it has no query
-  flash_loop(f, src, Images{k0, k1, v0, v1}, (k_end + Tile::KEYS - 1) / Tile::KEYS, qw >= len ? 0 : (qw + 31) / Tile::KEYS + 1, a.c);
-  const float inv = 1.0f / f.total();
-  if (qrow >= len) return;
-  T* op = (T*)a.o + (size_t)(seq + qrow) * a.o_ts + (size_t)head * a.o_hs;
-#pragma unroll
-  for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      u32x2 st = {cvt2<T>(f.o[dt][i] * inv, f.o[dt][i + 1] * inv), cvt2<T>(f.o[dt][i + 2] * inv, f.o[dt][i + 3] * inv)};
-      *(u32x2*)(op + dt * 32 + 2 * i + 4 * h) = st;
-    }
+  const Images im{k0, k1, v0, v1};
+  flash_loop(f, src, im, (k_end + Tile::KEYS - 1) / Tile::KEYS, qw >= len ? 0 : (qw + 31) / Tile::KEYS + 1, a.c);
+  T* op = (T*)a.o + (size_t)(seq + qw) * a.o_ts + (size_t)head * a.o_hs;
+  f.template rows<false>(im.of(w), lane, 1.0f / f.total(), [&](int row, int byte, u32x4 v) {
+    if (qw + row < len) *(u32x4*)((char*)(op + (size_t)row * a.o_ts) + byte) = v;
+  });
 }
 
 template <typename T, int HD> void launch_hd(const PackedArgs& a, hipStream_t s) {
@@ -136,8 +131,14 @@ extern "C" int orc_attn_plan(const int32_t* lens, int n, int32_t* out, int capac
   int at = 0, first = 0;
   for (int i = 0; i < n; first += lens[i], ++i)
     for (int q0 = 0; q0 < lens[i]; q0 += ROWS) w[at++] = int4{first, lens[i], q0, 0};
-  // a prompt's tiles together, so that its K / V are read from L2 by all of them; long prompts first, and in a prompt the tiles with the most keys
+  // A prompt's tiles together, so that its K / V are read from L2 by all of them; long prompts first, and in a prompt the tiles with the most keys.
+  // The last quarter of all tiles by their keys alone, so that no long one starts near the end (8 prompts of 640..900 tokens: all by prompt
+  // 65 us, the last quarter by keys 62, all by keys 76).
   std::sort(w, w + at, [](const int4& x, const int4& y) { return x.y != y.y ? x.y > y.y : x.x != y.x ? x.x < y.x : x.z > y.z; });
+  std::sort(w + at - at / 4, w + at, [](const int4& x, const int4& y) {
+    const int kx = std::min(x.z + ROWS, x.y), ky = std::min(y.z + ROWS, y.y);
+    return kx != ky ? kx > ky : x.x < y.x;
+  });
   return at;
 }
 

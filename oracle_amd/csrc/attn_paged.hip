@@ -355,18 +355,18 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
   const int tiles = (it.k_hi - it.k_lo + Tile64<HD>::KEYS - 1) / Tile64<HD>::KEYS;
   flash_loop(f, src, im, tiles, w * 32 < it.cols ? tiles : 0, a.c);   // a wave without columns helps with the loads
   const float sum = empty ? 0.f : f.total();
-  if (col < it.cols) {
-#pragma unroll
-    for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        put<T, HD>(a, it, col, dt * 32 + 2 * j + 4 * h, f.m, sum, f32x4{f.o[dt][j], f.o[dt][j + 1], f.o[dt][j + 2], f.o[dt][j + 3]});
-  }
+  // (with a prefix there are two parts at least: never the result itself)
+  const int at = (i * a.hq + it.kvh * a.group + fc % a.group) * (a.sp + a.ss) + it.part;
+  if (col < it.cols && h == 0) { a.ml[2 * (size_t)at] = f.m; a.ml[2 * (size_t)at + 1] = sum; }
+  f.template rows<true>(im.of(w), lane, 1.f, [&](int row, int byte, u32x4 v) {
+    const int to = __shfl(at, row, 64);
+    if (w * 32 + row < it.cols) *(u32x4*)((char*)(a.po + (size_t)to * HD) + byte) = v;
+  });
 }
 
 // PRE: how the prefix is read. 1, 2: keys_item with that many blocks of 16 columns; 8: cols_item, 128 columns
 template <typename T, int HD, int PRE>
-__global__ __launch_bounds__(256, PRE == 1 ? 4 : 2) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_kernel(AttendArgs a) {
   constexpr int QT = PRE == 8 ? 1 : PRE, MT = 16 * PRE, NID = PRE == 8 ? IDS_COLS : IDS;
   // a room holds a V tile, or the outputs of 16 QT columns; the tile images of cols_item are larger than either
   constexpr int V_TILE = KT * HD * 2, JOIN = MT * HD * 4, ROOM = PRE == 8 ? Tile64<HD>::BYTES : V_TILE > JOIN ? V_TILE : JOIN;

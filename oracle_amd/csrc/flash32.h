@@ -114,11 +114,40 @@ template <typename T, int HD> struct Flash32 {
     values(sV, pf);
   }
   __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
+
+  // The wave's 32 rows out of the registers, by way of LDS (room: 32 rows, nobody else's): a lane holds 4 values here and there of its row, and stored
+  // from there an instruction would touch 32 rows with 8 or 16 bytes each. store(row, byte, 16 bytes) is called for whole rows, the lanes of
+  // an instruction side by side. F32: the sums as they are; else times `inv`, rounded.
+  template <bool F32, typename Store> __device__ __forceinline__ void rows(char* room, int lane, float inv, Store store) const {
+    constexpr int RB = HD * (F32 ? 4 : 2), CHR = RB / 16, MASK = CHR < 16 ? CHR - 1 : 15;
+    const int q = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        if constexpr (F32) {
+          const int ch = dt * 8 + i / 2 + h;
+          *(f32x4*)(room + q * RB + ((ch ^ (q & MASK)) << 4)) = f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+        } else {
+          const int ch = dt * 4 + i / 4;
+          *(u32x2*)(room + q * RB + ((ch ^ (q & MASK)) << 4) + h * 8) =
+              u32x2{cvt2<T>(o[dt][i] * inv, o[dt][i + 1] * inv), cvt2<T>(o[dt][i + 2] * inv, o[dt][i + 3] * inv)};
+        }
+      }
+#pragma unroll
+    for (int x = 0; x < 32 * CHR / 64; ++x) {
+      const int row = x * (64 / CHR) + lane / CHR, ch = lane % CHR;
+      store(row, ch * 16, *(const u32x4*)(room + row * RB + ((ch ^ (row & MASK)) << 4)));
+    }
+  }
 };
 
 // The LDS images of even and odd tiles. Four arrays of their own, not one: the compiler then sees that a transposing read of one does not touch what the
 // DMA in flight writes, and does not wait for that DMA in front of it.
-struct Images { char *k0, *k1, *v0, *v1; };
+struct Images {
+  char *k0, *k1, *v0, *v1;
+  __device__ __forceinline__ char* of(int w) const { return w == 0 ? k0 : w == 1 ? k1 : w == 2 ? v0 : v1; }   // behind the loop: a wave's own
+};
 
 // The loop over the tiles of a workgroup of 4 waves, keys asked for two tiles ahead and values one. Iteration t waits for its values and the next
 // tile's keys, then a barrier (the waves are through with tile t - 1). The products of tile t + 1's scores stand between the exponentials of

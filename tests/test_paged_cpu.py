@@ -26,6 +26,8 @@ def test_plan_covers_every_row_once_and_runs_a_prompts_tiles_together(lib, lens)
     starts = np.cumsum([0] + lens).tolist()
     tile = 128
     want = [(s, x, q0, 0) for x, s in sorted(zip(lens, starts), key=lambda y: (-y[0], y[1])) for q0 in reversed(range(0, x, tile))]
+    last = n // 4       # these by their keys alone
+    want = want[:n - last] + sorted(want[n - last:], key=lambda y: (-min(y[2] + tile, y[1]), y[0]))
     assert [tuple(x) for x in work[:n].tolist()] == want
 
 
