@@ -38,22 +38,25 @@ def _chk(t, name, dim, dtype=None, device=None):
     if dtype is None:
         if t.dtype not in _DTYPES:
             raise ValueError(f'{name} must be bfloat16 or float16, got {t.dtype}')
-    elif t.dtype != dtype:
+    elif t.dtype is not dtype:
         raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
     if device is not None and t.device != device:
         raise ValueError(f'{name} is on {t.device}, not on {device}')
 
 
-def _strides(t, name):
-    """(token stride, head stride) of (tokens, heads, head_dim)"""
-    (n, heads, hd), (ts, hs, es) = t.shape, t.stride()
-    if es != 1 and hd > 1:
-        raise ValueError(f'{name}: the last dimension must be contiguous')
-    ts, hs = ts if n > 1 else 0, hs if heads > 1 else 0
-    if ts % 8 or hs % 8 or t.data_ptr() % 16:
-        raise ValueError(f'{name}: token and head strides must be multiples of 8 elements and the tensor must start on 16 bytes, '
-                         f'got strides {tuple(t.stride())} at {t.data_ptr() % 16} bytes past 16')
-    return ts, hs
+def _place(t, name):
+    """(token stride, head stride, address) of (tokens, heads, head_dim)"""
+    ts, hs, es = t.stride()
+    p = t.data_ptr()
+    if es != 1 or (ts | hs) & 7 or p & 15:
+        n, heads, hd = t.shape
+        ts, hs = ts if n > 1 else 0, hs if heads > 1 else 0      # the stride of one element does not matter
+        if es != 1 and hd > 1:
+            raise ValueError(f'{name}: the last dimension must be contiguous')
+        if (ts | hs) & 7 or p & 15:
+            raise ValueError(f'{name}: token and head strides must be multiples of 8 elements and the tensor must start on 16 bytes, '
+                             f'got strides {tuple(t.stride())} at {p % 16} bytes past 16')
+    return ts, hs, p
 
 
 def _overlaps_itself(t):
@@ -111,30 +114,34 @@ class PackedPlan:
 def packed_attention(q, k, v, plan, scale=None, out=None):
     """Causal attention inside every prompt of `plan`: q (T, Hq, hd), k / v (T, Hkv, hd) with T >= plan.total, hd 64 or 128, Hq a multiple of
     Hkv; slices of a fused projection are taken as they are. scale defaults to hd ** -0.5. Rows of `out` behind the last prompt are left
-    as they are (zero in a tensor made here)."""
+    as they are (zero in a tensor made here). `out` may be q, but must not lie over k or v."""
     _chk(q, 'q', 3)
-    _chk(k, 'k', 3, q.dtype, q.device)
-    _chk(v, 'v', 3, q.dtype, q.device)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    dtype, device = q.dtype, q.device
+    _chk(k, 'k', 3, dtype, device)
+    _chk(v, 'v', 3, dtype, device)
+    (tokens, hq, hd), (k_tokens, hkv, k_hd) = q.shape, k.shape
+    if k.shape != v.shape or k_tokens != tokens or k_hd != hd:
         raise ValueError(f'q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together')
-    hq, hkv, hd = q.shape[1], k.shape[1], q.shape[2]
     if hd not in (64, 128):
         raise ValueError(f'head_dim must be 64 or 128, got {hd}')
     if hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError(f'{hq} query heads are not a multiple of {hkv} K/V heads')
-    if plan.total > q.shape[0]:
-        raise ValueError(f'the plan covers {plan.total} tokens, q has {q.shape[0]}')
-    if plan.work.device != q.device:
-        raise ValueError(f'the plan is on {plan.work.device}, not on {q.device}')
+    if plan.total > tokens:
+        raise ValueError(f'the plan covers {plan.total} tokens, q has {tokens}')
+    if plan.work.device != device:
+        raise ValueError(f'the plan is on {plan.work.device}, not on {device}')
     scale = hd ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f'scale must be positive and finite, got {scale}')
     out = _out(out, q)
     if out is None:
-        out = (torch.empty if plan.total == q.shape[0] else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-    st = _I64x8(*_strides(q, 'q'), *_strides(k, 'k'), *_strides(v, 'v'), *_strides(out, 'out'))
-    _run(q.device, 'orc_attention_packed', q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st, plan.work.data_ptr(), plan.n_work, plan.total,
-         hq, hkv, hd, _DTYPES[q.dtype], scale)
+        out = (torch.empty if plan.total == tokens else torch.zeros)((tokens, hq, hd), dtype=dtype, device=device)
+    qt, qh, qp = _place(q, 'q')
+    kt, kh, kp = _place(k, 'k')
+    vt, vh, vp = _place(v, 'v')
+    ot, oh, op = _place(out, 'out')
+    _run(device, 'orc_attention_packed', qp, kp, vp, op, _I64x8(qt, qh, kt, kh, vt, vh, ot, oh), plan.work.data_ptr(), plan.n_work, plan.total,
+         hq, hkv, hd, _DTYPES[dtype], scale)
     return out
 
 
@@ -179,7 +186,8 @@ class KvPages:
         if n_pages * page > 0x7fffffff:
             raise ValueError('the pool holds more than 2^31 - 1 tokens')
         self.kv, self.table, self.lens, self.refs = kv, table, lens, refs
-        self.device, self.page_size, self.n_layers = kv.device, page, layers
+        self.device, self.dtype, self.n_layers, self.n_kv_heads, self.page_size, self.head_dim = kv.device, kv.dtype, layers, hkv, page, hd
+        self.row_tokens = table.shape[1] * page      # the most a row can hold
         self.status = torch.zeros(1, dtype=torch.int32, device=kv.device)
         self._work = torch.zeros(8 + 4 * n_pages, dtype=torch.int32, device=kv.device)
         self._c = _lib.OrcKvPages(*[t.data_ptr() for t in (kv, table, lens, refs, self.status, self._work)], layers, n_pages, hkv, page, hd,
@@ -221,23 +229,23 @@ class KvPages:
 
     def append(self, layer, slots, k, v):
         """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`; a place of -1 is skipped."""
-        _chk(k, 'k', 3, self.kv.dtype, self.device)
-        _chk(v, 'v', 3, self.kv.dtype, self.device)
-        want = (slots.numel(), self.kv.shape[3], self.kv.shape[5])
-        if tuple(k.shape) != want or tuple(v.shape) != want:
+        _chk(k, 'k', 3, self.dtype, self.device)
+        _chk(v, 'v', 3, self.dtype, self.device)
+        want = (slots.numel(), self.n_kv_heads, self.head_dim)
+        if k.shape != want or v.shape != want:
             raise ValueError(f'k {tuple(k.shape)} and v {tuple(v.shape)} must be {want}')
         self._layer(layer)
-        st = _I64x4(*_strides(k, 'k'), *_strides(v, 'v'))
-        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), slots.numel(), k.data_ptr(), v.data_ptr(), st)
+        (kt, kh, kp), (vt, vh, vp) = _place(k, 'k'), _place(v, 'v')
+        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), want[0], kp, vp, _I64x4(kt, kh, vt, vh))
 
     def _layer(self, layer):
         if not 0 <= layer < self.n_layers:
             raise ValueError(f'layer {layer} outside 0..{self.n_layers - 1}')
 
     def _fork(self, src, dst, n_tokens, share):
+        if n_tokens is not None and not 0 <= n_tokens <= 0x7fffffff:
+            raise ValueError(f'n_tokens must not be negative, got {n_tokens}')
         n_tokens = -1 if n_tokens is None else int(n_tokens)
-        if n_tokens < -1 or n_tokens > 0x7fffffff:
-            raise ValueError('n_tokens must not be negative')
         self._call('orc_kv_fork', self._rows(src, 'src'), self._rows(dst, 'dst', src.numel()), src.numel(), n_tokens, share)
 
     def fork(self, src, dst, n_tokens=None):
@@ -265,15 +273,14 @@ class KvPages:
         n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
         once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
         gives zeros."""
-        _chk(q, 'q', 3, self.kv.dtype, self.device)
+        _chk(q, 'q', 3, self.dtype, self.device)
         n, hq, hd = q.shape
-        if hd != self.kv.shape[5]:
-            raise ValueError(f'head_dim of q is {hd}, of the cache {self.kv.shape[5]}')
-        hkv = self.kv.shape[3]
-        if hq < 1 or hq % hkv:
-            raise ValueError(f'{hq} query heads are not a multiple of {hkv} K/V heads')
+        if hd != self.head_dim:
+            raise ValueError(f'head_dim of q is {hd}, of the cache {self.head_dim}')
+        if hq < 1 or hq % self.n_kv_heads:
+            raise ValueError(f'{hq} query heads are not a multiple of {self.n_kv_heads} K/V heads')
         self._layer(layer)
-        if prefix_tokens < 0 or prefix_tokens % self.page_size or prefix_tokens > self.table.shape[1] * self.page_size:
+        if not 0 <= prefix_tokens <= self.row_tokens or prefix_tokens % self.page_size:
             raise ValueError(f'prefix_tokens must be a multiple of page_size {self.page_size} inside a row, got {prefix_tokens}')
         r = self._rows(rows, n=n)
         lim = None if limits is None else _ints(limits, 'limits', self.device, n)
@@ -282,12 +289,11 @@ class KvPages:
             raise ValueError(f'scale must be positive and finite, got {scale}')
         out = _out(out, q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty((n, hq, hd), dtype=self.dtype, device=self.device)
         size = _lib.lib().orc_kv_attend_ws(self._ref, n, hq, int(prefix_tokens))
         if size < 0:
             _lib.check(-1, 'orc_kv_attend_ws')
         ws = torch.empty(size // 4, dtype=torch.float32, device=self.device) if size else None
-        st = _I64x4(*_strides(q, 'q'), *_strides(out, 'out'))
-        self._call('orc_kv_attend', int(layer), q.data_ptr(), out.data_ptr(), st, r, lim, n, hq, int(prefix_tokens), scale,
-                   ws.data_ptr() if size else None)
+        (qt, qh, qp), (ot, oh, op) = _place(q, 'q'), _place(out, 'out')
+        self._call('orc_kv_attend', int(layer), qp, op, _I64x4(qt, qh, ot, oh), r, lim, n, hq, int(prefix_tokens), scale, ws.data_ptr() if size else None)
         return out

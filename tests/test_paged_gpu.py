@@ -121,6 +121,8 @@ def test_packed_attention_layouts_stream_and_graph():
     heads_first = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)      # noqa: E731
     out = torch.empty(8, 123, 64, dtype=FP, device=DEV).transpose(0, 1)
     assert torch.equal(packed_attention(heads_first(q), heads_first(k), heads_first(v), plan, out=out), want)
+    inplace = q.clone()
+    assert torch.equal(packed_attention(inplace, k, v, plan, out=inplace), want)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -314,7 +316,7 @@ def test_refused_calls_change_nothing_and_say_why():
     m.same(c, 'a bad page')
     for bad in (lambda: c.reserve(torch.tensor([0], dtype=torch.int32)), lambda: c.reserve(torch.tensor([0], device=DEV)), lambda: c.reserve(ints([0]), ints([1])),
                 lambda: c.reserve(ints([0]), ints([1, 2]), total=3), lambda: c.reserve(ints([0]), total=-1), lambda: c.reserve(ints([[0]])),
-                lambda: c.reserve(ints(list(range(1025)))), lambda: c.fork(ints([0, 1]), ints([2])), lambda: c.fork(ints([0]), ints([2]), n_tokens=-2),
+                lambda: c.reserve(ints(list(range(1025)))), lambda: c.fork(ints([0, 1]), ints([2])), lambda: c.fork(ints([0]), ints([2]), n_tokens=-2), lambda: c.fork(ints([0]), ints([2]), n_tokens=-1),
                 lambda: c.append(2, ints([0]), *torch.zeros(2, 1, 2, 64, device=DEV, dtype=BF).unbind(0)),
                 lambda: c.append(0, ints([0]), *torch.zeros(2, 2, 2, 64, device=DEV, dtype=BF).unbind(0)),
                 lambda: c.append(0, ints([0]), *torch.zeros(2, 1, 2, 64, device=DEV, dtype=FP).unbind(0))):
