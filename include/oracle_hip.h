@@ -139,6 +139,12 @@ int orc_set_row_limits(orc_engine* e, const int32_t* limits_host, int n, void* s
 int orc_stream_begin(orc_engine* e, int n_rows, void* stream);
 int orc_prefill_slots(orc_engine* e, const int32_t* slots_host, int n, const void* embeds, const int32_t* position_ids,
                       const int32_t* left_pad_host, const int32_t* limits_host, int T, float* logits_out, void* stream);
+/* orc_prefill_slots for prompts of different lengths without padding: embeds (sum of lens_host, d_model), the prompts one behind the other, prompt i
+ * (lens_host[i] >= 1 tokens) from position 0 on into slot slots_host[i]; lens_host[i] + limits_host[i] <= max_seq. The projections run over
+ * the tokens there are, the attention through orc_attention_packed (which does not round the scores to bf16 on the way, as the padded
+ * form does in the reference's manner: results agree to bf16 tolerance, not bit by bit). */
+int orc_prefill_packed(orc_engine* e, const int32_t* slots_host, int n, const void* embeds, const int32_t* lens_host, const int32_t* limits_host,
+                       float* logits_out, void* stream);
 int orc_stream_attach(orc_engine* e, int row, int slot);
 int orc_read_slots(orc_engine* e, int32_t* tokens_host, int32_t* row_steps_host, int32_t* unfinished_host, void* stream);
 

@@ -114,7 +114,40 @@ template <typename T, int HD> void launch_hd(const PackedArgs& a, hipStream_t s)
   hipLaunchKernelGGL((packed_kernel<T, HD>), dim3((unsigned)(a.n_work * a.hq)), dim3(256), 0, s, a);
 }
 
+// The tiles of up to kMaxRows prompts, by prompt, written on the device; the prompts longest first, first: tiles before each of them
+struct PlanArgs { int n, first[kMaxRows + 1], start[kMaxRows], len[kMaxRows]; };
+__global__ __launch_bounds__(256) void plan_kernel(PlanArgs a, int4* work) {
+  for (int x = threadIdx.x; x < a.first[a.n]; x += 256) {
+    int i = 0;
+    while (i + 1 < a.n && x >= a.first[i + 1]) ++i;
+    work[x] = int4{a.start[i], a.len[i], (a.first[i + 1] - 1 - x) * ROWS, 0};
+  }
+}
+
 }  // namespace
+
+int attn_plan_ints(int rows) { return (rows / ROWS + kMaxRows) * 4; }
+
+int launch_attn_plan(const PackedRows& p, int32_t* work, hipStream_t s) {
+  if (p.n < 1 || p.n > kMaxRows) return orc_fail("launch_attn_plan", "1..32 prompts");
+  PlanArgs a;
+  int order[kMaxRows];
+  for (int i = 0; i < p.n; ++i) order[i] = i;
+  std::sort(order, order + p.n, [&](int x, int y) {
+    const int lx = p.start[x + 1] - p.start[x], ly = p.start[y + 1] - p.start[y];
+    return lx != ly ? lx > ly : x < y;
+  });
+  a.n = p.n;
+  a.first[0] = 0;
+  for (int i = 0; i < p.n; ++i) {
+    a.start[i] = p.start[order[i]];
+    a.len[i] = p.start[order[i] + 1] - a.start[i];
+    a.first[i + 1] = a.first[i] + (a.len[i] + ROWS - 1) / ROWS;
+  }
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(256), 0, s, a, (int4*)work);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? a.first[a.n] : orc_fail("launch_attn_plan", hipGetErrorString(e));
+}
 
 extern "C" int orc_attn_plan(const int32_t* lens, int n, int32_t* out, int capacity) {
   if (n < 0 || (n > 0 && !lens)) return orc_fail("orc_attn_plan", "null argument");

@@ -116,6 +116,7 @@ struct orc_engine {
   bf16_t *d_h = nullptr, *d_xn = nullptr, *d_qkv = nullptr, *d_att = nullptr, *d_mlp = nullptr;   // decode (<=16 rows)
   int *dev_ints = nullptr;   // [0]=step [2]=n_unfinished, then per-row arrays of 16 (DI_* offsets), then the token buffer
   int *d_step, *d_nunf, *d_unf, *d_next, *d_argmax, *d_kbeg, *d_kend, *d_rowoff, *d_rowvalid, *d_curlen, *d_rowstep, *d_limit, *d_tokens;
+  int32_t* d_plan = nullptr; // tile list of a packed prefill's attention
   int* d_pfkbeg = nullptr;   // [16] left pad of the rows of the prefill being launched (attention reads it per launch row)
   bool compress_decode = true;   // ORC_DECODE_WEIGHTS=plain turns the 12-bit decode copies off (A/B runs)
   // ORC_DECODE_NORM=exact: the decode path runs every RMSNorm as its own launch with the reference's rounding points (fp32
@@ -558,6 +559,7 @@ extern "C" int orc_engine_finalize(orc_engine* e) {
     ORCCHK(e->alloc((void**)&e->w_mlp, (size_t)rows * wm * 2));
     ORCCHK(e->alloc((void**)&e->w_logits, (size_t)kMaxRows * c.vocab * 4));
     ORCCHK(e->alloc((void**)&e->w_part, (size_t)kMaxRows * c.n_heads * DECODE_NSPLIT * 130 * 4));
+    ORCCHK(e->alloc((void**)&e->d_plan, (size_t)attn_plan_ints(rows) * 4));
     ORCCHK(e->alloc((void**)&e->d_ssq, (size_t)kMaxRows * (c.d_model / 16) * 4));
     ORCCHK(e->alloc((void**)&e->d_rowmeta, (size_t)kMaxRows * 4 * 4));
     ORCCHK(e->alloc((void**)&e->d_rowcos, (size_t)kMaxRows * 64 * 2));
@@ -764,11 +766,16 @@ static int gemv_ex(orc_engine* e, const bf16_t* X, int ldx, const Packed& W, con
 
 // prefill: tiled MFMA GEMMs + flash attention over all B*T positions
 // pm: batch row -> KV-cache slot the row is prefilled into. Leaves the final hidden state of the LAST position of every row in
-// d_h (B rows, row-major).
+// d_h (B rows, row-major). packed: the B prompts lie one behind the other instead (T, pos and pm are not used).
 static int llama_prefill_layers(orc_engine* e, bf16_t* h, bf16_t* xn, bf16_t* qkv, bf16_t* att, bf16_t* mlp, int B, int T,
-                                const int32_t* pos, hipStream_t s, const RowMap& pm) {
+                                const int32_t* pos, hipStream_t s, const RowMap& pm, const PackedRows* packed = nullptr) {
   const orc_config& c = e->c;
-  const int d = c.d_model, M = B * T;
+  const int d = c.d_model, M = packed ? packed->start[B] : B * T;
+  int n_work = 0;
+  if (packed) {
+    n_work = launch_attn_plan(*packed, e->d_plan, s);
+    if (n_work < 0) return -1;
+  }
   for (int i = 0; i < c.n_layers; ++i) {
     const LlamaLayer& L = e->llama[i];
     bf16_t* kc = e->kcache + (size_t)i * e->kv_layer_elems;
@@ -779,22 +786,33 @@ static int llama_prefill_layers(orc_engine* e, bf16_t* h, bf16_t* xn, bf16_t* qk
     r.qkv = qkv; r.B = B; r.T = T; r.H = c.n_heads; r.pos = pos; r.kbeg = e->d_kbeg; r.cur_len = e->d_curlen;
     r.cos_tab = e->cos_tab; r.sin_tab = e->sin_tab; r.maxpos = e->maxpos; r.Kc = kc; r.Vc = vc; r.c_bs = e->c_bs; r.c_hs = e->c_hs;
     r.t0 = 0; r.map = pm;
-    HIPCHK(launch_rope_kv(r, s));
-    AttnArgs a;
-    a.Q = qkv; a.q_bs = (long)T * 3 * d; a.q_hs = 128; a.q_ts = 3 * d;
-    a.K = kc; a.k_bs = e->c_bs; a.k_hs = e->c_hs; a.k_ts = 128;
-    a.V = vc; a.v_bs = e->c_bs; a.v_hs = e->c_hs; a.v_ts = 128;
-    a.O = att; a.o_bs = (long)T * d; a.o_hs = 128; a.o_ts = d;
-    a.B = B; a.H = c.n_heads; a.Sq = T; a.Sk = T; a.kbeg = e->d_pfkbeg; a.kend = nullptr; a.causal = 1; a.q_off = 0;
-    a.scale = 0.08838834764831845f;
-    a.kv_map_on = 1; a.kv_map = pm;
-    HIPCHK(launch_attention(a, 128, s));
+    if (packed) {
+      HIPCHK(launch_rope_packed(r, *packed, s));
+      const int64_t st[8] = {3 * d, 128, 3 * d, 128, 3 * d, 128, d, 128};
+      ORCCHK(orc_attention_packed(qkv, qkv + d, qkv + 2 * d, att, st, e->d_plan, n_work, M, c.n_heads, c.n_heads, 128, 0, 0.08838834764831845f, s));
+    } else {
+      HIPCHK(launch_rope_kv(r, s));
+      AttnArgs a;
+      a.Q = qkv; a.q_bs = (long)T * 3 * d; a.q_hs = 128; a.q_ts = 3 * d;
+      a.K = kc; a.k_bs = e->c_bs; a.k_hs = e->c_hs; a.k_ts = 128;
+      a.V = vc; a.v_bs = e->c_bs; a.v_hs = e->c_hs; a.v_ts = 128;
+      a.O = att; a.o_bs = (long)T * d; a.o_hs = 128; a.o_ts = d;
+      a.B = B; a.H = c.n_heads; a.Sq = T; a.Sk = T; a.kbeg = e->d_pfkbeg; a.kend = nullptr; a.causal = 1; a.q_off = 0;
+      a.scale = 0.08838834764831845f;
+      a.kv_map_on = 1; a.kv_map = pm;
+      HIPCHK(launch_attention(a, 128, s));
+    }
     if (i == c.n_layers - 1) {
       // Greedy search reads only the last position of every row (the reference computes logits for all T and discards them,
       // llava_llama.py:87-98), and nothing after the last layer's K / V write depends on the other positions: its o_proj and MLP
       // run on the B last rows only, through the decode GEMVs on the same packed weights (M = B <= 32).
-      HIPCHK(launch_copy_rows(att + (size_t)(T - 1) * d, (long)T * d, e->d_att, d, B, 1, d, s));
-      HIPCHK(launch_copy_rows(h + (size_t)(T - 1) * d, (long)T * d, e->d_h, d, B, 1, d, s));
+      if (packed) {
+        HIPCHK(launch_last_rows(att, *packed, e->d_att, d, s));
+        HIPCHK(launch_last_rows(h, *packed, e->d_h, d, s));
+      } else {
+        HIPCHK(launch_copy_rows(att + (size_t)(T - 1) * d, (long)T * d, e->d_att, d, B, 1, d, s));
+        HIPCHK(launch_copy_rows(h + (size_t)(T - 1) * d, (long)T * d, e->d_h, d, B, 1, d, s));
+      }
       ORCCHK(gemm(e->d_att, d, L.o, nullptr, e->d_h, d, e->d_h, d, B, EPI_RESIDUAL, s, true));
       HIPCHK(launch_rmsnorm(e->d_h, d, L.ln_post, e->d_xn, d, B, d, c.rms_eps, s));
       ORCCHK(gemm(e->d_xn, d, L.gu, nullptr, nullptr, 0, e->d_mlp, c.d_ff, B, EPI_SWIGLU, s, true));
@@ -885,13 +903,24 @@ static int head_and_sample(orc_engine* e, const bf16_t* hrows, int ldh, int B, f
 }
 
 // LlavaLlamaForCausalLM.forward step 0 for k left-padded rows into the KV-cache slots slots[0..k): resets those slots'
-// greedy state (one small launch, no host staging), runs the 32 layers over all k * T positions, samples each row's first token
+// greedy state (one small launch, no host staging), runs the 32 layers over all k * T positions, samples each row's first token.
+// lens: the rows' prompts lie one behind the other without padding instead, lens[i] rows each (position_ids, left_pad and T are not used).
 static int prefill_into_slots(orc_engine* e, const int* slots, int k, const void* embeds, const int32_t* position_ids,
-                              const int32_t* left_pad, const int32_t* limits, int T, float* logits_out, hipStream_t s, const char* who) {
+                              const int32_t* left_pad, const int32_t* limits, int T, float* logits_out, hipStream_t s, const char* who,
+                              const int32_t* lens = nullptr) {
   const orc_config& c = e->c;
   if (k < 1 || k > c.max_batch || k > kMaxRows) return fail(who, "row count outside 1..min(max_batch, 32)");
-  if (T < 1 || T >= c.max_seq) return fail(who, "prompt length exceeds max_seq");
-  if ((long)k * T > e->ws_rows) return fail(who, "rows*T exceeds workspace");
+  PackedRows pr = {};
+  if (lens) {
+    for (int i = 0; i < k; ++i) {
+      if (lens[i] < 1 || lens[i] >= c.max_seq) return fail(who, "prompt length outside 1..max_seq-1");
+      pr.start[i + 1] = pr.start[i] + lens[i];   // at most 32 x max_seq
+    }
+    pr.n = k;
+  } else if (T < 1 || T >= c.max_seq) {
+    return fail(who, "prompt length exceeds max_seq");
+  }
+  if ((lens ? (long)pr.start[k] : (long)k * T) > e->ws_rows) return fail(who, "rows*T exceeds workspace");
   SlotInitArgs in = {};
   RowMap pm;
   for (int i = 0; i < kMaxRows; ++i) pm.slot[i] = -1;
@@ -899,21 +928,24 @@ static int prefill_into_slots(orc_engine* e, const int* slots, int k, const void
     if (slots[i] < 0 || slots[i] >= c.max_batch) return fail(who, "slot outside 0..max_batch-1");
     for (int j = 0; j < i; ++j)
       if (slots[j] == slots[i]) return fail(who, "a slot is named twice");
-    if (left_pad[i] < 0 || left_pad[i] >= T) return fail(who, "left_pad outside 0..T-1");
+    if (lens) T = lens[i];
+    if (!lens && (left_pad[i] < 0 || left_pad[i] >= T)) return fail(who, "left_pad outside 0..T-1");
     const int lim = limits ? limits[i] : c.max_new_tokens;
     if (lim < 1 || lim > c.max_new_tokens) return fail(who, "length stop outside 1..max_new_tokens");
     if (limits && T + lim > c.max_seq) return fail(who, "prompt + length stop exceeds max_seq");
     pm.slot[i] = slots[i];
-    in.kbeg[i] = left_pad[i];
+    in.kbeg[i] = lens ? 0 : left_pad[i];
     in.limit[i] = lim;
+    in.T[i] = T;
   }
-  in.map = pm; in.k = k; in.T = T; in.pad_id = c.pad_token_id; in.out_ld = c.max_new_tokens;
+  pr.map = pm;
+  in.map = pm; in.k = k; in.pad_id = c.pad_token_id; in.out_ld = c.max_new_tokens;
   in.unfinished = e->d_unf; in.kbeg_state = e->d_kbeg; in.cur_len = e->d_curlen; in.row_step = e->d_rowstep; in.limit_state = e->d_limit;
   in.tokens = e->d_tokens; in.pf_kbeg = e->d_pfkbeg;
   HIPCHK(launch_slot_init(in, s));
-  const int d = c.d_model, M = k * T;
+  const int d = c.d_model, M = lens ? pr.start[k] : k * T;
   HIPCHK(hipMemcpyAsync(e->w_h, embeds, (size_t)M * d * 2, hipMemcpyDeviceToDevice, s));
-  ORCCHK(llama_prefill_layers(e, e->w_h, e->w_xn, e->w_qkv, e->w_att, e->w_mlp, k, T, position_ids, s, pm));
+  ORCCHK(llama_prefill_layers(e, e->w_h, e->w_xn, e->w_qkv, e->w_att, e->w_mlp, k, T, position_ids, s, pm, lens ? &pr : nullptr));
   ORCCHK(head_and_sample(e, e->d_h, d, k, logits_out, false, s, pm));   // the rows' last positions
   return 0;
 }
@@ -1042,6 +1074,18 @@ extern "C" int orc_prefill_slots(orc_engine* e, const int32_t* slots_host, int n
     for (int r = 0; r < e->cur_batch; ++r)
       if (e->row_map.slot[r] == slots_host[i]) return fail("orc_prefill_slots", "slot is attached to a decode row");
   return prefill_into_slots(e, slots_host, n, embeds, position_ids, left_pad_host, limits_host, T, logits_out, S(stream), "orc_prefill_slots");
+}
+
+extern "C" int orc_prefill_packed(orc_engine* e, const int32_t* slots_host, int n, const void* embeds, const int32_t* lens_host,
+                                  const int32_t* limits_host, float* logits_out, void* stream) {
+  const char* who = "orc_prefill_packed";
+  if (!e || !e->finalized) return fail(who, "engine not finalized");
+  if (!e->stream_mode) return fail(who, "call orc_stream_begin first");
+  if (!slots_host || !embeds || !lens_host || !limits_host) return fail(who, "null argument");
+  for (int i = 0; i < n && i < kMaxRows; ++i)
+    for (int r = 0; r < e->cur_batch; ++r)
+      if (e->row_map.slot[r] == slots_host[i]) return fail(who, "slot is attached to a decode row");
+  return prefill_into_slots(e, slots_host, n, embeds, nullptr, nullptr, limits_host, 0, logits_out, S(stream), who, lens_host);
 }
 
 extern "C" int orc_stream_attach(orc_engine* e, int row, int slot) {

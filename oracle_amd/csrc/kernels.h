@@ -18,6 +18,13 @@ struct RowMap {                 // default: row b <-> slot b
 };
 inline RowMap identity_map() { return RowMap(); }
 
+// Prompts packed one behind the other: rows [start[i], start[i + 1]) belong to prompt i, which goes to slot map.slot[i] from cache position 0 on
+struct PackedRows {
+  int n;
+  int start[kMaxRows + 1];
+  RowMap map;
+};
+
 enum { EPI_NONE = 0, EPI_QUICKGELU = 1, EPI_GELU = 2, EPI_RESIDUAL = 3, EPI_SWIGLU = 4, EPI_F32 = 5, EPI_ROPE_KV = 6 };
 
 struct GemmArgs {
@@ -155,6 +162,12 @@ struct RopeArgs {
   RowMap map;                 // batch row -> cache slot
 };
 hipError_t launch_rope_kv(const RopeArgs& a, hipStream_t s);
+// packed prompts: the position of a row is its place in its prompt; K is rotated in qkv too (the packed attention reads it there). a.B, a.T,
+// a.pos, a.t0 and a.map are not used.
+hipError_t launch_rope_packed(const RopeArgs& a, const PackedRows& p, hipStream_t s);
+// the tile list of orc_attention_packed for these prompts, on the device; returns its length (attn_packed.hip)
+int launch_attn_plan(const PackedRows& p, int32_t* work, hipStream_t s);
+int attn_plan_ints(int rows);   // ints a list for `rows` rows in up to kMaxRows prompts can take
 
 // ---- small data-movement kernels
 hipError_t launch_im2col(const bf16_t* img, int n_img, int image, int patch, bf16_t* out, int kp, hipStream_t s);
@@ -166,6 +179,8 @@ hipError_t launch_bert_embed(const bf16_t* feats, const int* row_off, const int*
 hipError_t launch_strip_cls(const bf16_t* h, bf16_t* out, int n_img, int tokens, int d, hipStream_t s);
 hipError_t launch_copy_rows(const bf16_t* src, long src_bs, bf16_t* dst, long dst_bs, int B, int rows, int d,
                             hipStream_t s);
+// out[i] = last row of packed prompt i
+hipError_t launch_last_rows(const bf16_t* src, const PackedRows& p, bf16_t* dst, int d, hipStream_t s);
 // splice: out[r][:] = kind==0 ? 0 : table_kind[idx][:]   (code = kind<<28 | idx)
 hipError_t launch_gather_rows(const int* codes, const bf16_t* tok, const bf16_t* img, const bf16_t* desc, bf16_t* out,
                               int rows, int d, hipStream_t s);
@@ -214,7 +229,8 @@ hipError_t launch_argmax_sample(const SampleArgs& a, hipStream_t s);
 struct SlotInitArgs {
   RowMap map; int k;                 // prefill row i -> slot
   int kbeg[kMaxRows]; int limit[kMaxRows];   // per prefill row: left pad, length stop
-  int T; int pad_id; int out_ld;
+  int T[kMaxRows];                   // per prefill row: cached keys
+  int pad_id; int out_ld;
   int *unfinished, *kbeg_state, *cur_len, *row_step, *limit_state, *tokens;   // per-slot state arrays
   int* pf_kbeg;                      // [kMaxRows] per prefill ROW copy of kbeg (read by the prefill attention)
 };

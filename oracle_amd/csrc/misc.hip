@@ -21,13 +21,24 @@ namespace {
 // One workgroup per token row; a work unit = (head, 8-element chunk c of the low half) handles elements
 // [8c, 8c+8) and their partners at +64 of q and k, plus the two v chunks.
 // q' = bf16( bf16(q*cos) + bf16(rotate_half(q)*sin) ), rotate_half(x) = cat(-x[64:], x[:64]).
-__global__ __launch_bounds__(256) void rope_kv_kernel(RopeArgs a) {
+template <bool PACKED>
+__global__ __launch_bounds__(256) void rope_kv_kernel(RopeArgs a, PackedRows p) {
   const int row = blockIdx.x;
-  const int b = row / a.T, t = row % a.T;
-  const int sl = a.map.slot[b];                 // KV-cache slot of this batch row
+  int b, t;
+  if constexpr (PACKED) {
+    b = 0;
+    while (b + 1 < p.n && row >= p.start[b + 1]) ++b;
+    t = row - p.start[b];
+  } else {
+    b = row / a.T;
+    t = row % a.T;
+  }
+  const int sl = PACKED ? p.map.slot[b] : a.map.slot[b];   // KV-cache slot of this batch row
   if (sl < 0) return;
   int pos, slot;
-  if (a.pos) {
+  if constexpr (PACKED) {
+    pos = slot = t;
+  } else if (a.pos) {
     pos = a.pos[row];
     slot = a.t0 + t;
   } else {
@@ -65,6 +76,10 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(RopeArgs a) {
       } else {
         *(u32x4*)(kdst + c * 8) = olo;
         *(u32x4*)(kdst + 64 + c * 8) = ohi;
+        if constexpr (PACKED) {
+          *(u32x4*)src = olo;
+          *(u32x4*)(src + 64) = ohi;
+        }
       }
     }
     *(u32x4*)(vdst + c * 8) = *(const u32x4*)(vr + head * 128 + c * 8);
@@ -136,6 +151,12 @@ __global__ __launch_bounds__(128) void strip_cls_kernel(const bf16_t* __restrict
   const int img = row / (tokens - 1), t = row % (tokens - 1);
   const bf16_t* src = h + ((size_t)img * tokens + t + 1) * d;
   for (int c = threadIdx.x; c < (d >> 3); c += 128) *(u32x4*)(out + (size_t)row * d + c * 8) = *(const u32x4*)(src + c * 8);
+}
+
+__global__ __launch_bounds__(128) void last_rows_kernel(const bf16_t* __restrict__ src, PackedRows p, bf16_t* __restrict__ dst, int d) {
+  const bf16_t* s = src + (size_t)(p.start[blockIdx.x + 1] - 1) * d;
+  bf16_t* o = dst + (size_t)blockIdx.x * d;
+  for (int c = threadIdx.x; c < (d >> 3); c += 128) *(u32x4*)(o + c * 8) = *(const u32x4*)(s + c * 8);
 }
 
 __global__ __launch_bounds__(128) void copy_rows_kernel(const bf16_t* __restrict__ src, long src_bs, bf16_t* __restrict__ dst,
@@ -352,7 +373,7 @@ __global__ __launch_bounds__(256) void slot_init_kernel(SlotInitArgs a) {
   if (threadIdx.x == 0) {
     a.unfinished[sl] = 1;
     a.kbeg_state[sl] = a.kbeg[i];
-    a.cur_len[sl] = a.T;
+    a.cur_len[sl] = a.T[i];
     a.row_step[sl] = 0;
     a.limit_state[sl] = a.limit[i];
     a.pf_kbeg[i] = a.kbeg[i];
@@ -373,7 +394,17 @@ inline int grid_for(size_t total) {
 
 hipError_t launch_rope_kv(const RopeArgs& a, hipStream_t s) {
   if (a.B * a.T <= 0) return hipSuccess;
-  hipLaunchKernelGGL(rope_kv_kernel, dim3(a.B * a.T), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(rope_kv_kernel<false>, dim3(a.B * a.T), dim3(256), 0, s, a, PackedRows{});
+  return hipGetLastError();
+}
+hipError_t launch_rope_packed(const RopeArgs& a, const PackedRows& p, hipStream_t s) {
+  if (p.n < 1 || p.n > kMaxRows || p.start[p.n] < 1) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(rope_kv_kernel<true>, dim3(p.start[p.n]), dim3(256), 0, s, a, p);
+  return hipGetLastError();
+}
+hipError_t launch_last_rows(const bf16_t* src, const PackedRows& p, bf16_t* dst, int d, hipStream_t s) {
+  if (p.n < 1 || p.n > kMaxRows) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(last_rows_kernel, dim3(p.n), dim3(128), 0, s, src, p, dst, d);
   return hipGetLastError();
 }
 hipError_t launch_im2col(const bf16_t* img, int n_img, int image, int patch, bf16_t* out, int kp, hipStream_t s) {

@@ -195,6 +195,19 @@ class Engine:
                                               _ptr(logits), _stream()), 'orc_prefill_slots')
         return logits
 
+    def prefill_packed(self, slots, embeds, lens, limits, want_logits=False):
+        """embeds (sum(lens), D) bf16: prompts of lens[i] tokens one behind the other, no padding, into the unattached KV slots `slots`; limits =
+        length stops."""
+        _chk_bf16(embeds, 'embeds')
+        n = len(slots)
+        if len(lens) != n or len(limits) != n or embeds.dim() != 2 or embeds.shape != (sum(int(x) for x in lens), self.dims.d_model):
+            raise ValueError(f'{n} slots, {len(lens)} lengths, {len(limits)} limits and embeds {tuple(embeds.shape)} do not belong together')
+        arr = lambda xs: (C.c_int32 * n)(*[int(x) for x in xs])
+        logits = torch.empty(n, self.dims.vocab, dtype=torch.float32, device=embeds.device) if want_logits else None
+        _lib.check(self.lib.orc_prefill_packed(self._h, arr(slots), n, _ptr(embeds), arr(lens), arr(limits), _ptr(logits), _stream()),
+                   'orc_prefill_packed')
+        return logits
+
     def stream_attach(self, row, slot):
         _lib.check(self.lib.orc_stream_attach(self._h, int(row), int(slot)), 'orc_stream_attach')
 

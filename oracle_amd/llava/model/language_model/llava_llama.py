@@ -210,7 +210,7 @@ class LlavaLlamaForCausalLM(LlavaMetaForCausalLM):
     # ------------------------------------------------------------------ continuous batching
     @torch.no_grad()
     def generate_stream(self, batches, max_new_tokens=20, n_rows=None, chunk=8, do_sample=False, use_cache=True,
-                        stopping_criteria=None):
+                        stopping_criteria=None, packed=False):
         """generate() over a stream of batches with continuous batching. The reference decodes batch
         after batch (scene_graph_prediction_model_oracle.py:251-260) and every batch runs as long as its longest answer;
         frames are independent, so here a decode row whose frame has finished (EOS / length stop) continues with the next
@@ -223,7 +223,11 @@ class LlavaLlamaForCausalLM(LlavaMetaForCausalLM):
         'limits': optional per-row length stops (synthetic workloads), 'stopping_criteria': optional, per batch}. Yields,
         in input order, what generate() returns for each batch: (B, L + n) = input_ids ++ new tokens, rows that finished
         early filled with pad, n = the longest row of that batch. A row's greedy tokens do not depend on its neighbours
-        (the decode GEMVs are bit-invariant to the batch), so the results equal generate() batch by batch."""
+        (the decode GEMVs are bit-invariant to the batch), so the results equal generate() batch by batch.
+
+        packed: frames that are prefilled together lie one behind the other instead of padded to the longest (Engine.prefill_packed): no work
+        for padding, and a frame's answer is bounded by its own length alone. The prefill's attention then keeps its scores in fp32, so
+        logits agree with generate() to bf16 tolerance, not bit by bit."""
         if do_sample:
             raise NotImplementedError('only greedy decoding (do_sample=False) is implemented, as ORacle uses')
         eng = self.engine
@@ -267,12 +271,13 @@ class LlavaLlamaForCausalLM(LlavaMetaForCausalLM):
             t = embeds.shape[1]
             for b in range(ids.shape[0]):
                 lim = max_new_tokens if limits is None else min(int(limits[b]), max_new_tokens)
-                if t + lim > eng.max_seq:      # t: the row may be prefilled at its batch's padded length
-                    if t >= eng.max_seq:
-                        raise ValueError(f'prompt ({t}) exceeds the KV capacity {eng.max_seq}')
-                    warnings.warn(f'prompt ({t}) + max_new_tokens ({lim}) exceeds the KV capacity {eng.max_seq}: '
-                                  f'generating at most {eng.max_seq - t} tokens')
-                    lim = eng.max_seq - t
+                held = counts[b] if packed else t      # t: the row may be prefilled at its batch's padded length
+                if held + lim > eng.max_seq:
+                    if held >= eng.max_seq:
+                        raise ValueError(f'prompt ({held}) exceeds the KV capacity {eng.max_seq}')
+                    warnings.warn(f'prompt ({held}) + max_new_tokens ({lim}) exceeds the KV capacity {eng.max_seq}: '
+                                  f'generating at most {eng.max_seq - held} tokens')
+                    lim = eng.max_seq - held
                 queue.append((next_in, b, embeds[b, t - counts[b]:], lim))
             info[next_in] = {'ids': ids, 'rows': {}, 'n': ids.shape[0], 'stopping': item.get('stopping_criteria', stopping_criteria)}
             next_in += 1
@@ -282,6 +287,10 @@ class LlavaLlamaForCausalLM(LlavaMetaForCausalLM):
             frames = [queue.pop(0) for _ in range(k)]
             slots = [free.pop(0) for _ in range(k)]
             lens = [f[2].shape[0] for f in frames]
+            if packed:
+                eng.prefill_packed(slots, torch.cat([f[2] for f in frames]), lens, [f[3] for f in frames])
+                waiting.extend((s_, f[0], f[1]) for s_, f in zip(slots, frames))
+                return
             t = max(lens)
             emb = torch.zeros(k, t, frames[0][2].shape[1], dtype=torch.bfloat16, device=frames[0][2].device)
             pos = torch.zeros(k, t, dtype=torch.int32)
