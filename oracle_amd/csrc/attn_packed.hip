@@ -46,17 +46,17 @@ template <typename T, int HD> struct PackedSrc {
     int left = len - t * Tile::KEYS;
     left = left < Tile::KEYS ? left : Tile::KEYS;
     const int bytes = (int)((left - 1) * ts + HD) * 2;
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long)t * Tile::KEYS * ts), 0, left > 0 ? bytes : 0, 0x00020000);
+    return buffer_of(base + (long)t * Tile::KEYS * ts, left > 0 ? bytes : 0);
   }
   __device__ __forceinline__ void next(int t) {
     kr = tile(kb, k_ts, t + 2);
     vr = tile(vb, v_ts, t + 1);
   }
   __device__ __forceinline__ void K(int, int r, char* to) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void_t*)(to + w * 1024 + r * 4096), 16, koff + (int)(r * KPR * k_ts * 2), 0, 0, 0);
+    buffer_load16_lds(kr, koff + (int)(r * KPR * k_ts * 2), to + w * 1024 + r * 4096);
   }
   __device__ __forceinline__ void V(int, int r, char* to) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void_t*)(to + w * 1024 + r * 4096), 16, voff + (int)(r * KPR * v_ts * 2), 0, 0, 0);
+    buffer_load16_lds(vr, voff + (int)(r * KPR * v_ts * 2), to + w * 1024 + r * 4096);
   }
   // Only a wave's last tile has keys in a query's future: tiles are 64 keys, the wave's queries 32 from a multiple of 32 on.
   __device__ __forceinline__ void mask_last(int t, f32x16 (&s)[2]) const {
@@ -101,9 +101,36 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_kernel(PackedArg
   Flash32<T, HD> f;
   f.init((const T*)a.q + (size_t)(seq + (qrow < len ? qrow : len - 1)) * a.q_ts + (size_t)head * a.q_hs, lane);
   const int k_end = q0 + ROWS < len ? q0 + ROWS : len;
-  // the wave's tiles: those behind are all in its future; 0: it has no query
   const Images im{k0, k1, v0, v1};
-  flash_loop(f, src, im, (k_end + Tile::KEYS - 1) / Tile::KEYS, qw >= len ? 0 : (qw + 31) / Tile::KEYS + 1, a.c);
+  const int tiles = (k_end + Tile::KEYS - 1) / Tile::KEYS;
+  const int mine = qw >= len ? 0 : (qw + 31) / Tile::KEYS + 1;   // the wave's tiles: those behind are all in its future; 0: it has no query
+  flash_loop(f, src, im, tiles, mine, a.c);
+  // A value that is infinite or NaN comes out where it was seen, and in the wave's last tile also where it was masked, as 0 times it. Told by the
+  // outputs, and done again one tile at a time with those values apart.
+  if (__syncthreads_or(!f.finite())) {
+    f.clear();
+    for (int t = 0; t < tiles; ++t) {
+      __syncthreads();
+      src.next(t - 2);
+#pragma unroll
+      for (int r = 0; r < src.RND; ++r) src.K(t, r, im.k0);
+      src.next(t - 1);
+#pragma unroll
+      for (int r = 0; r < src.RND; ++r) src.V(t, r, im.v0);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (t >= mine) continue;
+      f32x16 s[2] = {f.scores(im.k0, 0), f.scores(im.k0, 1)};
+      src.mask_last(t, s);
+      f.raise(f.largest(s), a.c);
+      const float mc = f.base(a.c);
+      u32x4 pf[4];
+      f.weights(s[0], a.c, mc, pf);
+      f.weights(s[1], a.c, mc, pf + 2);
+      f.values_careful(im.v0, pf, qrow - t * Tile::KEYS, lane >> 5);
+    }
+    __syncthreads();
+  }
   T* op = (T*)a.o + (size_t)(seq + qw) * a.o_ts + (size_t)head * a.o_hs;
   f.template rows<false>(im.of(w), lane, 1.0f / f.total(), [&](int row, int byte, u32x4 v) {
     if (qw + row < len) *(u32x4*)((char*)(op + (size_t)row * a.o_ts) + byte) = v;

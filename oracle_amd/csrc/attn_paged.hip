@@ -134,36 +134,38 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const T* kb = (const T*)a.k + (size_t)it.kvh * ps * HD + g * 8;
-  const T* vb = (const T*)a.v + (size_t)it.kvh * ps * HD;
+  const size_t head_off = (size_t)it.kvh * ps * ROWB, page_bytes = (size_t)a.page_elems * 2;
   char* sV = room.step ? room.r[0] + w * room.step : w == 0 ? room.r[0] : w == 1 ? room.r[1] : w == 2 ? room.r[2] : room.r[3];
   const int key_p = lane / CH, ch_p = lane % CH;
   for (int kc = it.k_lo; kc < it.k_hi; kc += (NID - 2) << a.log_ps) {
     const int first = kc >> a.log_ps, ke = kc + ((NID - 2) << a.log_ps) < it.k_hi ? kc + ((NID - 2) << a.log_ps) : it.k_hi;
     load_ids(a, it.row, first, ((ke - 1) >> a.log_ps) - first + 1, ids);
     for (int k0 = kc + w * KT; k0 < ke; k0 += 4 * KT) {
-      // the tile's two halves of 16 keys; one that is not there (behind the end, or its page outside the pool) loads a token of the other
-      const int i0 = (k0 >> a.log_ps) - first, i1 = k0 + 16 < ke ? ((k0 + 16) >> a.log_ps) - first : i0;
-      const int p0 = __builtin_amdgcn_readfirstlane(ids[i0]), p1 = k0 + 16 < ke ? __builtin_amdgcn_readfirstlane(ids[i1]) : -1;
+      // The tile's two halves of 16 keys, each on one page. The buffer descriptors end with the last token (at once, for a page outside the pool), so
+      // that what is not there arrives as zeros: its score is masked, and its value must not be something that 0 times it is not 0.
+      const bool two = k0 + 16 < ke;
+      const int p0 = __builtin_amdgcn_readfirstlane(ids[(k0 >> a.log_ps) - first]);
+      const int p1 = two ? __builtin_amdgcn_readfirstlane(ids[((k0 + 16) >> a.log_ps) - first]) : -1;
       if (p0 < 0 && p1 < 0) continue;
-      auto place = [&](int key) {   // element offset of a token of the tile
-        const bool up = key >= 16, there = up ? p1 >= 0 : p0 >= 0;
-        int at = k0 + key < ke ? k0 + key : ke - 1;
-        const int page = (up == there) ? p1 : p0;
-        if (!there) at = up ? k0 : k0 + 16;
-        return (size_t)page * a.page_elems + (size_t)((at & (ps - 1)) * HD);
-      };
-      v8 kf[2][HD / 32];
+      size_t off[2];
+      int at[2], bytes[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const T* kp = kb + place(b * 16 + c16);
-#pragma unroll
-        for (int kk = 0; kk < HD / 32; ++kk) kf[b][kk] = *(const v8*)(kp + kk * 32);
+        const int k = k0 + 16 * b, page = b ? p1 : p0;
+        at[b] = (k & (ps - 1)) * ROWB;
+        bytes[b] = page < 0 ? 0 : at[b] + (ke - k < 16 ? ke - k : 16) * ROWB;
+        off[b] = (size_t)(page < 0 ? 0 : page) * page_bytes + head_off;
       }
+      v8 kf[2][HD / 32];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk)
+          kf[b][kk] = __builtin_bit_cast(v8, buffer_load16(buffer_of(a.k + off[b], bytes[b]), at[b] + c16 * ROWB + g * 16 + kk * 64));
 #pragma unroll
       for (int r = 0; r < RND; ++r) {
-        const int key = r * KPR + key_p;
-        __builtin_amdgcn_global_load_lds((glb_void_t*)(vb + place(key) + swz_v16<HD>(key, ch_p) * 8), (lds_void_t*)(sV + r * 1024), 16, 0, 0);
+        const int key = r * KPR + key_p, b = r / (RND / 2);
+        buffer_load16_lds(buffer_of(a.v + off[b], bytes[b]), at[b] + (key - 16 * b) * ROWB + swz_v16<HD>(key, ch_p) * 16, sV + r * 1024);
       }
       f32x4 s[QT][2];
 #pragma unroll
@@ -306,13 +308,12 @@ template <typename T, int HD> struct PageSrc {
     const int k = (kc + (t + 3) * Tile::KEYS - 1) >> log_ps, v = (kc + (t + 1) * Tile::KEYS) >> log_ps;
     if (min(k - first, last) - win >= 64) window(min(v - first, last));
   }
-  // The r-th DMA instruction of tile t. A tile that begins or reaches behind the last token takes tokens of the last page instead: their
-  // scores are masked, or the tile is not read.
+  // The r-th DMA instruction of tile t; what lies behind the last token arrives as zeros (a descriptor of no bytes).
   __device__ __forceinline__ void ask(const char* base, unsigned l, int t, int r, char* to) const {
     const int k = kc + t * Tile::KEYS + r * KPR + w * GK, e = min((k >> log_ps) - first, last) - win;
     const unsigned long long off = (unsigned)__builtin_amdgcn_readlane((int)lo, e) | (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, e) << 32;
     const char* from = base + off + (unsigned)(k & ((1 << log_ps) - 1)) * (HD * 2);
-    __builtin_amdgcn_global_load_lds((glb_void_t*)(from + l), (lds_void_t*)(to + w * 1024 + r * 4096), 16, 0, 0);
+    buffer_load16_lds(buffer_of(from, k < ke ? GK * HD * 2 : 0), (int)l, to + w * 1024 + r * 4096);
   }
   __device__ __forceinline__ void K(int t, int r, char* to) const { ask(kb, lk, t, r, to); }
   __device__ __forceinline__ void V(int t, int r, char* to) const { ask(vb, lv, t, r, to); }

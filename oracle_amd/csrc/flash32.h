@@ -39,11 +39,13 @@ template <typename T, int HD> struct Flash32 {
       ka[kk] = c32 * Tile::ROWB + (Tile::swz_k(c32, kk * 2 + h) << 4);
     }
 #pragma unroll
-    for (int dt = 0; dt < HD / 32; ++dt) {
+    for (int dt = 0; dt < HD / 32; ++dt)
       va[dt] = vr * Tile::ROWB + (Tile::swz_v(vr, dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    }
+    for (int dt = 0; dt < HD / 32; ++dt) o[dt] = zero();
     m = -INFINITY;
     l = 0.f;
   }
@@ -103,6 +105,51 @@ template <typename T, int HD> struct Flash32 {
         o[dt] = Mma<T>::m32(join8<T>(lds_tr16<T>(p), lds_tr16<T>(p + 8 * Tile::ROWB)), p8, o[dt]);
       }
     }
+  }
+  // values() for a tile that may hold infinities or NaN where a query does not look: there 0 times the value would not be 0. Such values are left out of
+  // the product, and each one that a query sees (keys up to `sees` of the tile) marks its dim by what it adds: +inf, -inf, or both for NaN.
+  __device__ __forceinline__ void values_careful(const char* sV, const u32x4 (&pf)[4], int sees, int h) {
+    constexpr unsigned INF = Mma<T>::BF16 ? 0x7f80u : 0x7c00u, ONE = Mma<T>::BF16 ? 0x3f80u : 0x3c00u;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt) {
+      f32x16 up = zero(), down = zero();
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const char* p = sV + va[dt] + g * 16 * Tile::ROWB;
+        const u32x2 a = lds_tr16<T>(p), b = lds_tr16<T>(p + 8 * Tile::ROWB);
+        const u32x4 raw = {a[0], a[1], b[0], b[1]};
+        u32x4 clean, pu, pd, see;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          clean[j] = pu[j] = pd[j] = see[j] = 0;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const unsigned u = raw[j] >> (16 * x) & 0xffffu;
+            const bool odd = (u & INF) == INF, nan = odd && (u & 0x7fffu) != INF;
+            clean[j] |= (odd ? 0u : u) << (16 * x);
+            pu[j] |= (odd && (nan || !(u & 0x8000u)) ? ONE : 0u) << (16 * x);
+            pd[j] |= (odd && (nan || (u & 0x8000u)) ? ONE : 0u) << (16 * x);
+            see[j] |= (key_of(g >> 1, (g & 1) * 8 + 2 * j + x, h) <= sees ? ONE : 0u) << (16 * x);
+          }
+        }
+        o[dt] = Mma<T>::m32(__builtin_bit_cast(v8, clean), __builtin_bit_cast(v8, pf[g]), o[dt]);
+        up = Mma<T>::m32(__builtin_bit_cast(v8, pu), __builtin_bit_cast(v8, see), up);
+        down = Mma<T>::m32(__builtin_bit_cast(v8, pd), __builtin_bit_cast(v8, see), down);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (up[i] > 0.f) o[dt][i] += INFINITY;
+        if (down[i] > 0.f) o[dt][i] -= INFINITY;
+      }
+    }
+  }
+  __device__ __forceinline__ bool finite() const {
+    float z = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z = fmaf(o[dt][i], 0.f, z);
+    return z == 0.f;
   }
   // adds the tile: scores s (masked ones -inf), values at sV
   __device__ __forceinline__ void add(const char* sV, const f32x16 (&s)[2], float c) {

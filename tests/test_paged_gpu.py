@@ -113,6 +113,33 @@ def test_packed_attention_rows_behind_and_neighbours_do_not_matter():
         assert torch.equal(packed_attention(q, k2, v2, plan)[70:200], clean[70:200])
 
 
+@pytest.mark.parametrize('hd, dtype', [(128, BF), (64, FP)])
+def test_packed_attention_odd_values_reach_only_who_sees_them(hd, dtype):
+    lens, at = [200, 333], 200
+    q, k, v = qkv(sum(lens), 4, 2, hd, dtype, 40)
+    plan = PackedPlan(lens)
+    clean = packed_attention(q, k, v, plan)
+    inf, nan = float('inf'), float('nan')
+    for t, kh, d, value in ((0, 0, 3, inf), (63, 1, 0, nan), (64, 0, hd - 1, -inf), (131, 1, 40, inf), (332, 0, 7, nan), (300, 1, 33, -inf)):
+        odd = v.clone()
+        odd[at + t, kh, d] = value
+        out = packed_attention(q, k, odd, plan)
+        want = clean.clone()
+        want[at + t:, 2 * kh:2 * kh + 2, d] = value
+        seen = torch.zeros_like(want, dtype=torch.bool)
+        seen[at + t:, 2 * kh:2 * kh + 2, d] = True
+        assert torch.equal(out[seen].isnan(), want[seen].isnan()) and torch.equal(out[seen].nan_to_num(1, 2, 3), want[seen].nan_to_num(1, 2, 3)), (t, value)
+        close(out[~seen], clean[~seen].double(), torch.finfo(dtype).eps * clean[~seen].double().abs() + 2.0 ** -12, (t, value))
+    odd = v.clone()
+    odd[at + 10, 0, 5], odd[at + 100, 0, 5] = inf, -inf
+    out = packed_attention(q, k, odd, plan)
+    assert (out[at + 10:at + 100, :2, 5] == inf).all() and out[at + 100:, :2, 5].isnan().all() and torch.isfinite(out[at:at + 10]).all()
+    odd = k.clone()
+    odd[at + 150, 1] = nan
+    out = packed_attention(q, odd, v, plan)
+    assert out[at + 150:, 2:].isnan().all() and torch.isfinite(out[:at + 150]).all() and torch.isfinite(out[:, :2]).all()
+
+
 def test_packed_attention_layouts_stream_and_graph():
     lens = [90, 33]
     q, k, v = qkv(123, 8, 4, 64, FP, 5)
@@ -438,6 +465,21 @@ def test_attend_limits_rows_named_often_and_rows_outside():
         n = min(n, dense[r][0].shape[1])
         ref, tol = attention64(q[i], dense[r][0][:, :n], dense[r][1][:, :n], 0.3)
         close(out[i], ref, tol, (i, r, n))
+
+
+@pytest.mark.parametrize('n, hq, hkv', [(2, 4, 2), (6, 8, 2), (40, 8, 2)])
+def test_attend_odd_values_come_out_as_they_are(n, hq, hkv):
+    c, _ = filled(n, 96, [5 + i % 7 for i in range(n)], 32, hkv, 64, FP, 50 + n)
+    rows = ints(list(range(n)))
+    q = torch.randn(n, hq, 64, device=DEV).to(FP)
+    clean = c.attend(1, q, rows, prefix_tokens=96)
+    page, g = int(c.table[0, 2]), hq // hkv
+    for value in (float('inf'), float('-inf'), float('nan')):
+        c.kv[1, 1, page, 1, 31, 9] = value            # the prefix's last token
+        out = c.attend(1, q, rows, prefix_tokens=96)
+        odd = torch.zeros_like(out, dtype=torch.bool)
+        odd[:, g:2 * g, 9] = True
+        assert (out[odd].isnan().all() if value != value else (out[odd] == value).all()) and torch.equal(out[~odd], clean[~odd])
 
 
 def test_attend_many_columns_and_wide_groups():
