@@ -103,12 +103,12 @@ __device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col
   }
 }
 
-// LDS of keys_item: a V tile for each wave and, behind the loop, the waves' maxima, sums and outputs, in the same four rooms. step: their distance in
+// LDS of keys_item: a V tile for each wave and, behind the loop, its outputs, in the wave's own room. step: the rooms' distance in
 // one array (picking a room by address arithmetic takes fewer registers, and 128 are the limit), 0 where they are arrays of their own.
 struct Rooms { char* r[4]; int step; };
 
 template <typename T, int HD, int QT, int NID>
-__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids) {
+__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
   typedef typename Mma<T>::v8 v8;
   constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH, MT = 16 * QT;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
@@ -223,57 +223,32 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
     }
   }
 
-  // join the four waves: maxima and sums of all, then the outputs of waves 2, 3 into 0, 1 and of 1 into 0
-  __syncthreads();
-  float* sm = (float*)room.r[0];             // [4][MT] maxima, [4][MT] sums
-  float* so = (float*)(w & 1 ? room.r[2] : room.r[1]);   // [MT][HD] of a pair of waves
+  // Join the four waves: each leaves its maxima, sums and outputs (in its own room, 16-byte pieces permuted against bank conflicts); behind one
+  // barrier every thread adds up its pieces of the columns.
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
     l[t] += __shfl_xor(l[t], 32, 64);
     if (g == 0) { sm[w * MT + t * 16 + c16] = m[t]; sm[(4 + w) * MT + t * 16 + c16] = l[t]; }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) *(f32x4*)(sV + (t * 16 + c16) * HD * 4 + (((d * 4 + g) ^ c16) << 4)) = o[t][d];
   }
   __syncthreads();
-  float mx[QT], sum[QT];
+  for (int x = threadIdx.x; x < it.cols * (HD / 4); x += 256) {
+    const int col = x / (HD / 4), d4 = x % (HD / 4);
+    float mx = -INFINITY, sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int col = t * 16 + c16;
-    mx[t] = -INFINITY; sum[t] = 0.f;
+    for (int y = 0; y < 4; ++y) mx = fmaxf(mx, sm[y * MT + col]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) mx[t] = fmaxf(mx[t], sm[x * MT + col]);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float lx = sm[(4 + x) * MT + col];
-      if (lx != 0.f) sum[t] += lx * __builtin_amdgcn_exp2f((sm[x * MT + col] - mx[t]) * a.c);
+    for (int y = 0; y < 4; ++y) {
+      const float ly = sm[(4 + y) * MT + col], f = __builtin_amdgcn_exp2f((sm[y * MT + col] - mx) * a.c);
+      if (ly != 0.f) {            // a wave without keys for this column: nothing to add (its maximum is -inf)
+        sum += ly * f;
+        v += *(const f32x4*)(room.r[y] + col * HD * 4 + ((d4 ^ (col & 15)) << 4)) * f;
+      }
     }
-    const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - mx[t]) * a.c);
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) o[t][d] = l[t] != 0.f ? o[t][d] * f : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-#pragma unroll
-  for (int half = 2; half >= 1; half >>= 1) {
-    if (w >= half && w < 2 * half) {
-      float* to = half == 2 ? so : (float*)room.r[1];   // wave 3 to 1, 2 to 0; then 1 to 0
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) *(f32x4*)(to + (size_t)(t * 16 + c16) * HD + d * 16 + 4 * g) = o[t][d];
-    }
-    __syncthreads();
-    if (w < half) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[t][d] += *(const f32x4*)(so + (size_t)(t * 16 + c16) * HD + d * 16 + 4 * g);
-    }
-    __syncthreads();
-  }
-  if (w == 0) {
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-      if (t * 16 + c16 < it.cols)
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) put<T, HD>(a, it, t * 16 + c16, d * 16 + 4 * g, mx[t], sum[t], o[t][d]);
+    put<T, HD>(a, it, col, d4 * 4, mx, sum, v);
   }
 }
 
@@ -327,7 +302,7 @@ template <typename T, int HD> struct PageSrc {
 };
 
 template <typename T, int HD>
-__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, const Images& im, int* ids) {
+__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, const Images& im, int* ids, float* sm) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int ps = 1 << a.log_ps, col = w * 32 + (lane & 31);
   const int fc = it.f0 + (col < it.cols ? col : 0), i = fc / a.group;
@@ -341,7 +316,7 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
     for (int x = 0; x < it.cols; x += 16) {
       sub.f0 = it.f0 + x;
       sub.cols = it.cols - x < 16 ? it.cols - x : 16;
-      keys_item<T, HD, 1, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids);
+      keys_item<T, HD, 1, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids, sm);
     }
     return;
   }
@@ -375,6 +350,7 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
   __shared__ __attribute__((aligned(16))) char r0[PRE == 8 ? ROOM : 4 * ROOM], r1[ONE], r2[ONE], r3[ONE];
   const Rooms room = PRE == 8 ? Rooms{{r0, r1, r2, r3}, 0} : Rooms{{r0, r0 + ROOM, r0 + 2 * ROOM, r0 + 3 * ROOM}, ROOM};
   __shared__ int ids[NID];
+  __shared__ float sm[8 * 16 * QT];      // the waves' maxima and sums
   // The prefix's items come first, the rows' own tokens behind them. (Taking turns in groups of 8 was slower, by up to 2x: workgroups are dealt round
   // robin to an XCD's shader engines, so a regular pattern of long and short ones loads some engines with the long ones.)
   const int lane = threadIdx.x & 63, pairs = a.hkv * a.sp, n_pre = pairs * a.mt;
@@ -395,8 +371,8 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
     it.f0 = mt * MT;
     it.cols = a.n * a.group - it.f0;
     if (it.cols > MT) it.cols = MT;
-    if constexpr (PRE == 8) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids);
-    else keys_item<T, HD, QT, NID>(a, it, room, ids);
+    if constexpr (PRE == 8) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids, sm);
+    else keys_item<T, HD, QT, NID>(a, it, room, ids, sm);
     return;
   }
   it.kvh = x % a.hkv; x /= a.hkv;
@@ -418,7 +394,7 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
   it.f0 = i * a.group + gt * 16;
   it.cols = a.group - gt * 16;
   if (it.cols > 16) it.cols = 16;
-  keys_item<T, HD, 1, NID>(a, it, room, ids);
+  keys_item<T, HD, 1, NID>(a, it, room, ids, sm);
 }
 
 // One wave per (query, head): lane s holds the weight of part s; then the lanes hold the head's dims, 16 bytes each, and a wave reads 64 * 4 / HD
