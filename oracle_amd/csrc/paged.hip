@@ -96,8 +96,9 @@ __device__ int check_rows(const Pages& p, const int* rows, int n, unsigned* seen
   return bad;
 }
 
+// all threads' bits together
 __device__ int block_or(int v, int* sh) {
-  __syncthreads();
+  if (!__syncthreads_or(v)) return 0;
   if (threadIdx.x == 0) sh[0] = 0;
   __syncthreads();
   if (v) atomicOr(&sh[0], v);
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(NT) void fork_kernel(Pages p, const int* src, const
     }
   }
   const int used = pages_of(p, len), keep = share ? len >> p.log_ps : 0;
-  atomicMax(&most_sh, used);
+  if (used) atomicMax(&most_sh, used);   // (1024 threads on one LDS word would take 2 us)
   bad = block_or(bad, sh);
   int need_all = 0, at = 0;
   if (!bad) at = block_scan(used - keep, &need_all, sh);
