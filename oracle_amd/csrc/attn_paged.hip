@@ -6,7 +6,7 @@
 // combine_kernel joins the parts of a query by exp2(c (m_part - m)).
 //
 // Two shapes of work, 4 waves each:
-//   keys_item  few query columns (16 or 32: one row's heads over its own tokens, or a small batch over the prefix): the waves share the columns and
+//   keys_item  16 query columns (one row's heads over its own tokens, or a small batch over the prefix): the waves share the columns and
 //              split the keys. A wave's tile is 32 keys, K straight to registers in operand order, V through 8 KiB of LDS of its own; no
 //              barrier in the loop and little LDS, so 4 workgroups fit a CU and hide each other's memory latency. Bound by HBM.
 //   cols_item  many columns over the prefix: every wave has 32 columns of its own, 64-key tiles go through a 2-deep LDS ring that
@@ -107,33 +107,27 @@ __device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col
 // one array (picking a room by address arithmetic takes fewer registers, and 128 are the limit), 0 where they are arrays of their own.
 struct Rooms { char* r[4]; int step; };
 
-template <typename T, int HD, int QT, int NID>
+template <typename T, int HD, int NID>
 __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
   typedef typename Mma<T>::v8 v8;
-  constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH, MT = 16 * QT;
+  constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
-  const int ps = 1 << a.log_ps, nq = (it.cols + 15) >> 4;
-  int lim_c[QT];                  // the lane's query columns: c16 of every block of 16
-  v8 qf[QT][HD / 32];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int col = t * 16 + c16;
-    const int f = it.f0 + (col < it.cols ? col : 0), i = f / a.group, head = it.kvh * a.group + f % a.group;
+  const int ps = 1 << a.log_ps;
+  int lim;                        // of the lane's query column c16
+  v8 qf[HD / 32];
+  {
+    const int f = it.f0 + (c16 < it.cols ? c16 : 0), i = f / a.group, head = it.kvh * a.group + f % a.group;
     int r;
-    const int lim = visible(a, i, &r);
-    lim_c[t] = col < it.cols ? (lim < it.k_hi ? lim : it.k_hi) : 0;
+    lim = visible(a, i, &r);
+    lim = c16 < it.cols ? (lim < it.k_hi ? lim : it.k_hi) : 0;
     const T* qp = (const T*)a.q + (size_t)i * a.q_ts + (size_t)head * a.q_hs + g * 8;
 #pragma unroll
-    for (int kk = 0; kk < HD / 32; ++kk) qf[t][kk] = *(const v8*)(qp + kk * 32);
+    for (int kk = 0; kk < HD / 32; ++kk) qf[kk] = *(const v8*)(qp + kk * 32);
   }
-  f32x4 o[QT][HD / 16];
-  float m[QT], l[QT];
+  f32x4 o[HD / 16];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY; l[t] = 0.f;
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   const size_t head_off = (size_t)it.kvh * ps * ROWB, page_bytes = (size_t)a.page_elems * 2;
   char* sV = room.step ? room.r[0] + w * room.step : w == 0 ? room.r[0] : w == 1 ? room.r[1] : w == 2 ? room.r[2] : room.r[3];
   const int key_p = lane / CH, ch_p = lane % CH;
@@ -167,46 +161,35 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
         const int key = r * KPR + key_p, b = r / (RND / 2);
         buffer_load16_lds(buffer_of(a.v + off[b], bytes[b]), at[b] + (key - 16 * b) * ROWB + swz_v16<HD>(key, ch_p) * 16, sV + r * 1024);
       }
-      f32x4 s[QT][2];
+      f32x4 s[2];
+      float tm = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
+        s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kk = 0; kk < HD / 32; ++kk) s[b] = Mma<T>::m16(kf[b][kk], qf[kk], s[b]);
 #pragma unroll
-        for (int kk = 0; kk < HD / 32; ++kk)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            if (t < nq) s[t][b] = Mma<T>::m16(kf[b][kk], qf[t][kk], s[t][b]);
-      }
-      v8 pf[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        if (t >= nq) continue;
-        float tm = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool see = k0 + b * 16 + 4 * g + r < lim_c[t] && (b ? p1 : p0) >= 0;
-            s[t][b][r] = see ? s[t][b][r] : -INFINITY;
-            tm = fmaxf(tm, s[t][b][r]);
-          }
-        tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-        tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-        const float m_new = fmaxf(m[t], tm), mu = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f((m[t] - mu) * a.c);
-        m[t] = m_new;
-        l[t] *= alpha;
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[t][d] *= alpha;
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          p[j] = __builtin_amdgcn_exp2f((s[t][j >> 2][j & 3] - mu) * a.c);
-          l[t] += p[j];
+        for (int r = 0; r < 4; ++r) {
+          const bool see = k0 + b * 16 + 4 * g + r < lim && (b ? p1 : p0) >= 0;
+          s[b][r] = see ? s[b][r] : -INFINITY;
+          tm = fmaxf(tm, s[b][r]);
         }
-        pf[t] = __builtin_bit_cast(v8, (u32x4){cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])});
       }
+      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+      tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+      const float m_new = fmaxf(m, tm), mu = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f((m - mu) * a.c);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f((s[j >> 2][j & 3] - mu) * a.c);
+        l += p[j];
+      }
+      const v8 pf = __builtin_bit_cast(v8, (u32x4){cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])});
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // V is in LDS
       const int key = 4 * g + (c16 >> 2);
 #pragma unroll
@@ -214,10 +197,7 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
         const int ch = d * 2 + ((lane & 3) >> 1);
         const u32x2 v0 = lds_tr16<T>(sV + key * ROWB + (swz_v16<HD>(key, ch) << 4) + (lane & 1) * 8);
         const u32x2 v1 = lds_tr16<T>(sV + (key + 16) * ROWB + (swz_v16<HD>(key + 16, ch) << 4) + (lane & 1) * 8);
-        const v8 vf = join8<T>(v0, v1);
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-          if (t < nq) o[t][d] = Mma<T>::m16(vf, pf[t], o[t][d]);
+        o[d] = Mma<T>::m16(join8<T>(v0, v1), pf, o[d]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile's reads are done before the next tile's DMA
     }
@@ -225,27 +205,24 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
 
   // Join the four waves: each leaves its maxima, sums and outputs (in its own room, 16-byte pieces permuted against bank conflicts); behind one
   // barrier every thread adds up its pieces of the columns.
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) { sm[w * 16 + c16] = m; sm[(4 + w) * 16 + c16] = l; }
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    l[t] += __shfl_xor(l[t], 16, 64);
-    l[t] += __shfl_xor(l[t], 32, 64);
-    if (g == 0) { sm[w * MT + t * 16 + c16] = m[t]; sm[(4 + w) * MT + t * 16 + c16] = l[t]; }
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) *(f32x4*)(sV + (t * 16 + c16) * HD * 4 + (((d * 4 + g) ^ c16) << 4)) = o[t][d];
-  }
+  for (int d = 0; d < HD / 16; ++d) *(f32x4*)(sV + c16 * HD * 4 + (((d * 4 + g) ^ c16) << 4)) = o[d];
   __syncthreads();
   for (int x = threadIdx.x; x < it.cols * (HD / 4); x += 256) {
     const int col = x / (HD / 4), d4 = x % (HD / 4);
     float mx = -INFINITY, sum = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int y = 0; y < 4; ++y) mx = fmaxf(mx, sm[y * MT + col]);
+    for (int y = 0; y < 4; ++y) mx = fmaxf(mx, sm[y * 16 + col]);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const float ly = sm[(4 + y) * MT + col], f = __builtin_amdgcn_exp2f((sm[y * MT + col] - mx) * a.c);
+      const float ly = sm[(4 + y) * 16 + col], f = __builtin_amdgcn_exp2f((sm[y * 16 + col] - mx) * a.c);
       if (ly != 0.f) {            // a wave without keys for this column: nothing to add (its maximum is -inf)
         sum += ly * f;
-        v += *(const f32x4*)(room.r[y] + col * HD * 4 + ((d4 ^ (col & 15)) << 4)) * f;
+        v += *(const f32x4*)(room.r[y] + col * HD * 4 + ((d4 ^ col) << 4)) * f;
       }
     }
     put<T, HD>(a, it, col, d4 * 4, mx, sum, v);
@@ -316,7 +293,7 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
     for (int x = 0; x < it.cols; x += 16) {
       sub.f0 = it.f0 + x;
       sub.cols = it.cols - x < 16 ? it.cols - x : 16;
-      keys_item<T, HD, 1, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids, sm);
+      keys_item<T, HD, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids, sm);
     }
     return;
   }
@@ -340,19 +317,17 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
   });
 }
 
-// PRE: how the prefix is read. 1, 2: keys_item with that many blocks of 16 columns; 8: cols_item, 128 columns
-template <typename T, int HD, int PRE>
-__global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_kernel(AttendArgs a) {
-  constexpr int QT = PRE == 8 ? 1 : PRE, MT = 16 * PRE, NID = PRE == 8 ? IDS_COLS : IDS;
-  // a room holds a V tile, or the outputs of 16 QT columns; the tile images of cols_item are larger than either
-  constexpr int V_TILE = KT * HD * 2, JOIN = MT * HD * 4, ROOM = PRE == 8 ? Tile64<HD>::BYTES : V_TILE > JOIN ? V_TILE : JOIN;
-  constexpr int ONE = PRE == 8 ? ROOM : 16;
-  __shared__ __attribute__((aligned(16))) char r0[PRE == 8 ? ROOM : 4 * ROOM], r1[ONE], r2[ONE], r3[ONE];
-  const Rooms room = PRE == 8 ? Rooms{{r0, r1, r2, r3}, 0} : Rooms{{r0, r0 + ROOM, r0 + 2 * ROOM, r0 + 3 * ROOM}, ROOM};
+// COLS: the prefix is read by cols_item, 128 query columns at a time; else by keys_item, 16
+template <typename T, int HD, bool COLS>
+__global__ __launch_bounds__(256, COLS ? (HD == 64 ? 3 : 2) : 4) void attend_kernel(AttendArgs a) {
+  constexpr int MT = COLS ? 128 : 16, NID = COLS ? IDS_COLS : IDS;
+  // a room holds a V tile of 32 keys, or 16 columns' outputs (as much); the tile images of cols_item are larger
+  constexpr int ROOM = COLS ? Tile64<HD>::BYTES : KT * HD * 2, ONE = COLS ? ROOM : 16;
+  static_assert(16 * HD * 4 <= KT * HD * 2, "the outputs fit the V tile");
+  __shared__ __attribute__((aligned(16))) char r0[COLS ? ROOM : 4 * ROOM], r1[ONE], r2[ONE], r3[ONE];
+  const Rooms room = COLS ? Rooms{{r0, r1, r2, r3}, 0} : Rooms{{r0, r0 + ROOM, r0 + 2 * ROOM, r0 + 3 * ROOM}, ROOM};
   __shared__ int ids[NID];
-  __shared__ float sm[8 * 16 * QT];      // the waves' maxima and sums
-  // The prefix's items come first, the rows' own tokens behind them. (Taking turns in groups of 8 was slower, by up to 2x: workgroups are dealt round
-  // robin to an XCD's shader engines, so a regular pattern of long and short ones loads some engines with the long ones.)
+  __shared__ float sm[8 * 16];           // the waves' maxima and sums
   const int lane = threadIdx.x & 63, pairs = a.hkv * a.sp, n_pre = pairs * a.mt;
   int x = (int)blockIdx.x - n_pre;
   Item it;
@@ -363,7 +338,7 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
     else { pair = p_at / a.mt; mt = p_at % a.mt; }
     it.kvh = pair % a.hkv;
     it.part = pair / a.hkv;
-    constexpr int UNIT = PRE == 8 ? Tile64<HD>::KEYS : KT;
+    constexpr int UNIT = COLS ? Tile64<HD>::KEYS : KT;
     const int per = ((a.prefix + UNIT - 1) / UNIT + a.sp - 1) / a.sp * UNIT;
     it.k_lo = it.part * per;
     it.k_hi = it.k_lo + per < a.prefix ? it.k_lo + per : a.prefix;
@@ -371,8 +346,8 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
     it.f0 = mt * MT;
     it.cols = a.n * a.group - it.f0;
     if (it.cols > MT) it.cols = MT;
-    if constexpr (PRE == 8) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids, sm);
-    else keys_item<T, HD, QT, NID>(a, it, room, ids, sm);
+    if constexpr (COLS) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids, sm);
+    else keys_item<T, HD, NID>(a, it, room, ids, sm);
     return;
   }
   it.kvh = x % a.hkv; x /= a.hkv;
@@ -394,7 +369,7 @@ __global__ __launch_bounds__(256, PRE == 1 ? 4 : HD == 64 ? 3 : 2) void attend_k
   it.f0 = i * a.group + gt * 16;
   it.cols = a.group - gt * 16;
   if (it.cols > 16) it.cols = 16;
-  keys_item<T, HD, 1, NID>(a, it, room, ids, sm);
+  keys_item<T, HD, NID>(a, it, room, ids, sm);
 }
 
 // One wave per (query, head): lane s holds the weight of part s; then the lanes hold the head's dims, 16 bytes each, and a wave reads 64 * 4 / HD
@@ -444,26 +419,32 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
 }
 
 // how a call is split; the same for the scratch size and the launch
-struct Split { int pre, mt, gt, sp, ss; };
+struct Split { bool cols; int mt, gt, sp, ss; };
 Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   Split s;
   const int group = n_heads / c->n_kv_heads;
   const int64_t cols = (int64_t)n * group;
-  // cols_item reads at most IDS_COLS - 4 pages, 40 parts at the most
+  // keys_item reads the prefix once for every 16 columns, cols_item for every 128, with fewer and larger workgroups. The second pass of 17 to 32
+  // columns is cheap while the first one's pages are in the caches (keys / cols us at 32 columns: 32 K/V heads, 768 shared tokens 18.3 / 20.8, 4k
+  // 28.2 / 30.6; 2 heads, 16k 17.4 / 20.9) and is not beyond (32 heads, 8k, 134 MB 42.9 / 43.2; 16k 71.9 / 66.0); more passes cost more (48
+  // columns: 8 heads, 4k 15.3 / 15.6, 32k 52.2 / 39.1; 32 heads, 8k 60.3 / 51.1).
+  // cols_item reads at most IDS_COLS - 4 pages, of 40 parts at the most.
   const int64_t range = (int64_t)(IDS_COLS - 4) * c->page_size, least_sp = (prefix + range - 1) / range;
-  s.pre = cols <= 16 ? 1 : cols <= 32 || least_sp > 40 ? 2 : 8;
-  s.mt = prefix ? (int)((cols + 16 * s.pre - 1) / (16 * s.pre)) : 0;
+  const int64_t bytes = (int64_t)prefix * c->n_kv_heads * c->head_dim * 4;
+  s.cols = cols > (bytes > 128 << 20 ? 16 : 32) && least_sp <= 40;
+  const int wide = s.cols ? 128 : 16;
+  s.mt = prefix ? (int)((cols + wide - 1) / wide) : 0;
   s.gt = (group + 15) / 16;
   s.sp = 0;
   if (prefix) {
     const int64_t base = (int64_t)c->n_kv_heads * s.mt;
     // cols_item runs two to a CU: 384 items leave every fourth place to the rows' own tokens, which are bound by memory (96 rows, 4 heads a
     // K/V head, 32k + 570 tokens: 264 items 131 us, 384 136, 504 143; without own tokens 96, 86, 87). keys_item: 512, of 256 keys and more.
-    int64_t sp = ((s.pre == 8 ? 384 : 512) + base - 1) / base;
+    int64_t sp = ((s.cols ? 384 : 512) + base - 1) / base;
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
     sp = sp < 1 ? 1 : sp > 40 ? 40 : sp;
-    s.sp = (int)(s.pre == 8 && sp < least_sp ? least_sp : sp);
+    s.sp = (int)(s.cols && sp < least_sp ? least_sp : sp);
   }
   const int64_t own = (int64_t)n * c->n_kv_heads * s.gt;
   const int64_t left = (int64_t)c->max_row_pages * c->page_size - prefix;
@@ -486,15 +467,15 @@ const char* bad_call(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   return nullptr;
 }
 
-template <typename T, int HD, int PRE> hipError_t launch_pre(const AttendArgs& a, hipStream_t s) {
+template <typename T, int HD, bool COLS> hipError_t launch_cols(const AttendArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)(a.hkv * a.mt * a.sp + a.n * a.hkv * a.gt * a.ss);
-  hipLaunchKernelGGL((attend_kernel<T, HD, PRE>), dim3(grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attend_kernel<T, HD, COLS>), dim3(grid), dim3(256), 0, s, a);
   if (a.sp + a.ss > 1)
     hipLaunchKernelGGL((combine_kernel<T, HD>), dim3((unsigned)(((int64_t)a.n * a.hq + 3) / 4)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
-template <typename T, int HD> hipError_t launch_hd(const AttendArgs& a, int pre, hipStream_t s) {
-  return pre == 1 ? launch_pre<T, HD, 1>(a, s) : pre == 2 ? launch_pre<T, HD, 2>(a, s) : launch_pre<T, HD, 8>(a, s);
+template <typename T, int HD> hipError_t launch_hd(const AttendArgs& a, bool cols, hipStream_t s) {
+  return cols ? launch_cols<T, HD, true>(a, s) : launch_cols<T, HD, false>(a, s);
 }
 
 }  // namespace
@@ -537,7 +518,7 @@ extern "C" int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, vo
   a.c = scale * 1.4426950408889634f;
   hipStream_t hs = (hipStream_t)stream;
   hipError_t e;
-  if (c->dtype == 0) e = c->head_dim == 128 ? launch_hd<__bf16, 128>(a, s.pre, hs) : launch_hd<__bf16, 64>(a, s.pre, hs);
-  else e = c->head_dim == 128 ? launch_hd<_Float16, 128>(a, s.pre, hs) : launch_hd<_Float16, 64>(a, s.pre, hs);
+  if (c->dtype == 0) e = c->head_dim == 128 ? launch_hd<__bf16, 128>(a, s.cols, hs) : launch_hd<__bf16, 64>(a, s.cols, hs);
+  else e = c->head_dim == 128 ? launch_hd<_Float16, 128>(a, s.cols, hs) : launch_hd<_Float16, 64>(a, s.cols, hs);
   return e == hipSuccess ? 0 : orc_fail(who, hipGetErrorString(e));
 }
