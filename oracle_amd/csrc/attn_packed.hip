@@ -210,7 +210,7 @@ extern "C" int orc_attention_packed(const void* q, const void* k, const void* v,
   if (head_dim != 64 && head_dim != 128) return orc_fail(who, "head_dim is 64 or 128");
   if (dtype != 0 && dtype != 1) return orc_fail(who, "dtype is 0 (bf16) or 1 (fp16)");
   if (!(scale > 0.f) || !(scale < 1e30f)) return orc_fail(who, "scale is not positive and finite");
-  if ((int64_t)n_work * n_heads > 0x7fffffff) return orc_fail(who, "too many tiles");
+  if ((int64_t)n_work * n_heads > 0xffffff) return orc_fail(who, "too many tiles: with the heads 2^24 - 1 at the most");   // 256 threads each: 32 bits
   for (int i = 0; i < 8; ++i)
     if (st[i] < 0 || st[i] % 8) return orc_fail(who, "strides are not multiples of 8 elements");
   if (st[2] >= 1 << 24 || st[4] >= 1 << 24) return orc_fail(who, "K / V token strides of 2^24 elements and more");   // a tile's offsets are 32-bit

@@ -263,19 +263,34 @@ __global__ __launch_bounds__(256) void copy_kernel(const char* from, char* to, c
 __global__ __launch_bounds__(NT) void free_kernel(Pages p, const int* rows, int n) {
   __shared__ int sh[NT / 64 + 1];
   __shared__ unsigned seen[2048];
+  __shared__ int pages[NT], most_sh;
+  const int t = threadIdx.x;
+  if (t == 0) most_sh = 0;
   int bad = check_rows(p, rows, n, seen);
   bad = block_or(bad, sh);
   if (bad) {
-    if (threadIdx.x == 0) atomicOr(p.status, bad);
+    if (t == 0) atomicOr(p.status, bad);
     return;
   }
-  for (long x = threadIdx.x; x < (long)n * p.width; x += NT) {
-    int* e = &p.table[(size_t)rows[x / p.width] * p.width + x % p.width];
+  // Up to the longest row, not the table's width (64 rows of 13 pages in a table 4096 wide: 108 -> 7 us; of 2000: 186 -> 51; 16 of 13 in 16: 6.2 -> 6.7).
+  int used = 0;   // the row's pages
+  if (t < n) {
+    const int len = p.lens[rows[t]];
+    used = len <= 0 ? 0 : len < p.width * p.ps ? pages_of(p, len) : p.width;
+    if (used) atomicMax(&most_sh, used);
+  }
+  pages[t] = used;
+  __syncthreads();
+  const int most = most_sh;
+  for (int x = t; x < n * most; x += NT) {
+    const int i = x / most, j = x - i * most;
+    if (j >= pages[i]) continue;
+    int* e = &p.table[(size_t)rows[i] * p.width + j];
     const int page = *e;
     if (page >= 0 && page < p.n_pages) atomicSub(&p.refs[page], 1);
     *e = -1;
   }
-  for (int i = threadIdx.x; i < n; i += NT) p.lens[rows[i]] = 0;
+  if (t < n) p.lens[rows[t]] = 0;
 }
 
 // where every held page goes: map[page] (work list 3) and the copies; in place only pages behind the last to keep move
@@ -364,6 +379,7 @@ Pages dev(const orc_kv_pages* c) {
   p.max_rows = c->max_rows; p.width = c->max_row_pages; p.head_bytes = c->head_dim * 2;
   return p;
 }
+bool overlap(const void* x, int64_t nx, const void* y, int64_t ny) { return (const char*)x < (const char*)y + ny && (const char*)y < (const char*)x + nx; }
 int done(const char* who) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : orc_fail(who, hipGetErrorString(e));
@@ -435,7 +451,11 @@ extern "C" int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, v
     if (into->n_layers != c->n_layers || into->n_kv_heads != c->n_kv_heads || into->page_size != c->page_size || into->head_dim != c->head_dim ||
         into->dtype != c->dtype || into->max_rows != c->max_rows || into->max_row_pages != c->max_row_pages)
       return orc_fail(who, "the caches differ in more than n_pages");
-    if (into->kv == c->kv || into->table == c->table || into->lens == c->lens || into->refs == c->refs) return orc_fail(who, "the caches share memory");
+    const int64_t page = (int64_t)c->n_layers * 2 * c->n_kv_heads * c->page_size * c->head_dim * 2;
+    if (overlap(into->kv, into->n_pages * page, c->kv, c->n_pages * page) || overlap(into->refs, into->n_pages * 4ll, c->refs, c->n_pages * 4ll) ||
+        overlap(into->table, c->max_rows * 4ll * c->max_row_pages, c->table, c->max_rows * 4ll * c->max_row_pages) ||
+        overlap(into->lens, c->max_rows * 4ll, c->lens, c->max_rows * 4ll))
+      return orc_fail(who, "the caches share memory");
   }
   const Pages p = dev(c), q = in_place ? p : dev(into);
   hipStream_t s = (hipStream_t)stream;

@@ -1,7 +1,7 @@
 """Prompts of different lengths in one pass, and a paged KV cache: attention over packed prompts (`packed_attention`), and `KvPages` --
 pages taken and filled (`reserve`, `append`), shared and copied (`fork`, `copy`), given back (`free`), moved together (`compact`), and
 decode attention that reads a prefix shared by the whole batch once (`attend`). The C entry points are orc_attention_packed and
-orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it."""
+orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it. There are no gradients."""
 import ctypes as C
 
 import torch
@@ -42,6 +42,8 @@ def _chk(t, name, dim, dtype=None, device=None):
         raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
     if device is not None and t.device != device:
         raise ValueError(f'{name} is on {t.device}, not on {device}')
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f'{name} requires a gradient and the call has none: detach it, or call under torch.no_grad()')
 
 
 def _place(t, name):
@@ -228,15 +230,16 @@ class KvPages:
         return slots
 
     def append(self, layer, slots, k, v):
-        """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`; a place of -1 is skipped."""
+        """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`, each named once; a place of -1 is skipped."""
         _chk(k, 'k', 3, self.dtype, self.device)
         _chk(v, 'v', 3, self.dtype, self.device)
+        s = _ints(slots, 'slots', self.device)
         want = (slots.numel(), self.n_kv_heads, self.head_dim)
         if k.shape != want or v.shape != want:
             raise ValueError(f'k {tuple(k.shape)} and v {tuple(v.shape)} must be {want}')
         self._layer(layer)
         (kt, kh, kp), (vt, vh, vp) = _place(k, 'k'), _place(v, 'v')
-        self._call('orc_kv_append', int(layer), _ints(slots, 'slots', self.device), want[0], kp, vp, _I64x4(kt, kh, vt, vh))
+        self._call('orc_kv_append', int(layer), s, want[0], kp, vp, _I64x4(kt, kh, vt, vh))
 
     def _layer(self, layer):
         if not 0 <= layer < self.n_layers:
@@ -263,7 +266,8 @@ class KvPages:
 
     def compact(self, into=None):
         """Held pages to the front of the pool: in place, the pages that stick out move into the holes. into: another cache of the same geometry
-        (n_pages may differ), which becomes a copy of this one without the holes; this one stays as it is."""
+        (n_pages may differ), which becomes a copy of this one without the holes; this one stays as it is. Too few pages there: a note that
+        into.check() raises, and nothing is changed."""
         if into is not None and into.device != self.device:
             raise ValueError(f'into is on {into.device}, not on {self.device}')
         self._call('orc_kv_compact', None if into is None else into._ref)
@@ -272,7 +276,7 @@ class KvPages:
         """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
         n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
         once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
-        gives zeros."""
+        gives zeros; what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q."""
         _chk(q, 'q', 3, self.dtype, self.device)
         n, hq, hd = q.shape
         if hd != self.head_dim:

@@ -53,7 +53,7 @@ PACKED_OK = dict(st=[1024, 128] * 4, n_work=1, total=4, hq=8, hkv=8, hd=128, dty
     (dict(hq=9), b'multiple'), (dict(hkv=0), b'multiple'), (dict(hd=96), b'head_dim'), (dict(dtype=2), b'dtype'),
     (dict(scale=0.0), b'scale'), (dict(scale=float('nan')), b'scale'), (dict(scale=-1.0), b'scale'), (dict(scale=float('inf')), b'scale'),
     (dict(st=[1020] + [1024] * 7), b'strides'), (dict(st=[-8] + [1024] * 7), b'strides'), (dict(ptr=0), b'null'), (dict(ptr=4104), b'aligned'),
-    (dict(n_work=-1), b'bad'), (dict(n_work=1 << 30), b'too many')])
+    (dict(n_work=-1), b'bad'), (dict(n_work=1 << 30), b'too many'), (dict(n_work=1 << 21), b'too many')])
 def test_packed_attention_refusals_of_the_c_entry(lib, change, text):
     a = dict(PACKED_OK, **change)
     st = (C.c_int64 * 8)(*a['st'])
@@ -105,6 +105,7 @@ def test_call_refusals_of_the_c_entries(lib):
     refused(lib.orc_kv_fork(c, None, 4096, 1, -1, 1, None), b'null')
     refused(lib.orc_kv_free(c, 4096, -1, None), b'1024')
     refused(lib.orc_kv_compact(c, c, None), b'share memory')
+    refused(lib.orc_kv_compact(c, C.byref(cache(kv=8192, table=1 << 21, lens=1 << 22, refs=1 << 23)), None), b'share memory')   # the pool is 64 KiB
     refused(lib.orc_kv_compact(c, C.byref(cache(kv=1 << 20, table=1 << 21, lens=1 << 22, refs=1 << 23, page_size=32)), None), b'differ')
 
     def attend(**change):

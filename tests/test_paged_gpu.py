@@ -72,7 +72,7 @@ def test_packed_attention(lens, hq, hkv, hd, dtype):
     close(out, ref, tol, lens)
 
 
-def test_packed_attention_long_enough_for_the_tall_tiles():
+def test_packed_attention_long_prompts():
     lens = [4200, 3900, 77]
     for hd, dtype in ((128, BF), (64, FP)):
         q, k, v = qkv(sum(lens), 16, 2, hd, dtype, 2)
