@@ -107,19 +107,24 @@ __device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col
 // one array (picking a room by address arithmetic takes fewer registers, and 128 are the limit), 0 where they are arrays of their own.
 struct Rooms { char* r[4]; int step; };
 
+// Up to 16 columns. True where a value that some column does not see may have spoilt an output (it is infinite or NaN, and 0 times it is not 0).
 template <typename T, int HD, int NID>
-__device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
+__device__ __forceinline__ bool keys_item(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
   typedef typename Mma<T>::v8 v8;
   constexpr int ROWB = HD * 2, CH = HD / 8, TILE = KT * ROWB, RND = TILE / 1024, KPR = 64 / CH;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));   // what follows from it is computed here, not held in registers around the loop of keys_items
+  const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c16 = lane & 15;
   const int ps = 1 << a.log_ps;
   int lim;                        // of the lane's query column c16
+  bool part;
   v8 qf[HD / 32];
   {
     const int f = it.f0 + (c16 < it.cols ? c16 : 0), i = f / a.group, head = it.kvh * a.group + f % a.group;
     int r;
     lim = visible(a, i, &r);
     lim = c16 < it.cols ? (lim < it.k_hi ? lim : it.k_hi) : 0;
+    part = __any(lim > it.k_lo && lim < it.k_hi);   // (the waves hold the same columns)
     const T* qp = (const T*)a.q + (size_t)i * a.q_ts + (size_t)head * a.q_hs + g * 8;
 #pragma unroll
     for (int kk = 0; kk < HD / 32; ++kk) qf[kk] = *(const v8*)(qp + kk * 32);
@@ -189,8 +194,9 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
         p[j] = __builtin_amdgcn_exp2f((s[j >> 2][j & 3] - mu) * a.c);
         l += p[j];
       }
-      const v8 pf = __builtin_bit_cast(v8, (u32x4){cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])});
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // V is in LDS
+      u32x4 pw = {cvt2<T>(p[0], p[1]), cvt2<T>(p[2], p[3]), cvt2<T>(p[4], p[5]), cvt2<T>(p[6], p[7])};
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(pw)::"memory");   // V is in LDS. (With pw: otherwise the wait may move in front of the scores.)
+      const v8 pf = __builtin_bit_cast(v8, pw);
       const int key = 4 * g + (c16 >> 2);
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) {
@@ -211,7 +217,8 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
 #pragma unroll
   for (int d = 0; d < HD / 16; ++d) *(f32x4*)(sV + c16 * HD * 4 + (((d * 4 + g) ^ c16) << 4)) = o[d];
   __syncthreads();
-  for (int x = threadIdx.x; x < it.cols * (HD / 4); x += 256) {
+  bool odd = false;
+  for (int x = tid; x < it.cols * (HD / 4); x += 256) {
     const int col = x / (HD / 4), d4 = x % (HD / 4);
     float mx = -INFINITY, sum = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -226,6 +233,32 @@ __device__ __forceinline__ void keys_item(const AttendArgs& a, const Item& it, c
       }
     }
     put<T, HD>(a, it, col, d4 * 4, mx, sum, v);
+    odd |= !(fmaf(v[0], 0.f, v[1] * 0.f) + fmaf(v[2], 0.f, v[3] * 0.f) == 0.f);
+  }
+  return part && __builtin_amdgcn_readfirstlane(__syncthreads_or(odd));   // a scalar: a loop around it stays one of the whole wave
+}
+
+// The item's columns, 16 at a time; where a value that not all of them see is infinite or NaN, again one by one, up to the column's last token.
+template <typename T, int HD, int NID>
+__device__ __forceinline__ void keys_items(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
+  Item sub = it;
+  int x = 0, wide = 16, back = 0;
+  while (x < it.cols) {
+    sub.f0 = it.f0 + x;
+    sub.cols = it.cols - x < wide ? it.cols - x : wide;
+    sub.k_hi = it.k_hi;
+    if (wide == 1) {
+      int r;
+      const int lim = visible(a, sub.f0 / a.group, &r);
+      sub.k_hi = lim < it.k_hi ? lim : it.k_hi;
+    }
+    if (keys_item<T, HD, NID>(a, sub, room, ids, sm)) {
+      back = x + sub.cols;
+      wide = 1;
+      continue;
+    }
+    x += sub.cols;
+    if (x == back) wide = 16;
   }
 }
 
@@ -278,8 +311,10 @@ template <typename T, int HD> struct PageSrc {
   }
 };
 
+// Up to 128 columns. False, and nothing done, where a page is outside the pool or a query ends before the item's keys do: keys_items has a test for
+// every key.
 template <typename T, int HD>
-__device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, const Images& im, int* ids, float* sm) {
+__device__ __forceinline__ bool cols_item(const AttendArgs& a, const Item& it, const Images& im, int* ids) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int ps = 1 << a.log_ps, col = w * 32 + (lane & 31);
   const int fc = it.f0 + (col < it.cols ? col : 0), i = fc / a.group;
@@ -287,16 +322,7 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
   const int lim = visible(a, i, &r);
   const bool empty = lim == 0;             // a column whose query has no tokens (a row that has ended): what it computes is not used
   const int first = it.k_lo >> a.log_ps;
-  if (load_ids(a, it.row, first, ((it.k_hi - 1) >> a.log_ps) - first + 1, ids, lim > 0 && lim < it.k_hi)) {
-    // a page outside the pool, or a query that ends before the prefix does: 16 columns at a time, where every key has its test
-    Item sub = it;
-    for (int x = 0; x < it.cols; x += 16) {
-      sub.f0 = it.f0 + x;
-      sub.cols = it.cols - x < 16 ? it.cols - x : 16;
-      keys_item<T, HD, IDS_COLS>(a, sub, Rooms{{im.k0, im.k1, im.v0, im.v1}, 0}, ids, sm);
-    }
-    return;
-  }
+  if (load_ids(a, it.row, first, ((it.k_hi - 1) >> a.log_ps) - first + 1, ids, lim > 0 && lim < it.k_hi)) return false;
   PageSrc<T, HD> src;
   src.kb = a.k + (size_t)it.kvh * ps * HD * 2;
   src.vb = a.v + (size_t)it.kvh * ps * HD * 2;
@@ -315,6 +341,7 @@ __device__ __forceinline__ void cols_item(const AttendArgs& a, const Item& it, c
     const int to = __shfl(at, row, 64);
     if (w * 32 + row < it.cols) *(u32x4*)((char*)(a.po + (size_t)to * HD) + byte) = v;
   });
+  return true;
 }
 
 // COLS: the prefix is read by cols_item, 128 query columns at a time; else by keys_item, 16
@@ -346,30 +373,30 @@ __global__ __launch_bounds__(256, COLS ? (HD == 64 ? 3 : 2) : 4) void attend_ker
     it.f0 = mt * MT;
     it.cols = a.n * a.group - it.f0;
     if (it.cols > MT) it.cols = MT;
-    if constexpr (COLS) cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids, sm);
-    else keys_item<T, HD, NID>(a, it, room, ids, sm);
-    return;
+    if constexpr (COLS)
+      if (cols_item<T, HD>(a, it, Images{r0, r1, r2, r3}, ids)) return;
+  } else {
+    it.kvh = x % a.hkv; x /= a.hkv;
+    const int gt = x % a.gt; x /= a.gt;
+    const int sx = x % a.ss, i = x / a.ss;
+    const int lim = visible(a, i, &it.row);
+    if (a.prefix && it.kvh == 0 && gt == 0 && sx == 0 && threadIdx.x < 64 && it.row >= 0) {   // what it reads as shared, is it on the same pages?
+      const int pr = prefix_row(a, lane), held = ((lim < a.prefix ? lim : a.prefix) + (1 << a.log_ps) - 1) >> a.log_ps;
+      bool differ = false;
+      for (int j = lane; j < held; j += 64) differ |= pr < 0 || a.table[(size_t)it.row * a.width + j] != a.table[(size_t)pr * a.width + j];
+      if (__any(differ) && lane == 0) atomicOr(a.status, (int)ORC_KV_NOT_SHARED);
+    }
+    const int tiles = (lim - a.prefix + KT - 1) / KT;
+    int per = (tiles + a.ss - 1) / a.ss;
+    per = (per < 4 ? 4 : per) * KT;   // at least a tile for each wave
+    it.k_lo = a.prefix + sx * per;
+    it.k_hi = it.k_lo + per < lim ? it.k_lo + per : lim;
+    it.part = a.sp + sx;
+    it.f0 = i * a.group + gt * 16;
+    it.cols = a.group - gt * 16;
+    if (it.cols > 16) it.cols = 16;
   }
-  it.kvh = x % a.hkv; x /= a.hkv;
-  const int gt = x % a.gt; x /= a.gt;
-  const int sx = x % a.ss, i = x / a.ss;
-  const int lim = visible(a, i, &it.row);
-  if (a.prefix && it.kvh == 0 && gt == 0 && sx == 0 && threadIdx.x < 64 && it.row >= 0) {   // what it reads as shared, is it on the same pages?
-    const int pr = prefix_row(a, lane), held = ((lim < a.prefix ? lim : a.prefix) + (1 << a.log_ps) - 1) >> a.log_ps;
-    bool differ = false;
-    for (int j = lane; j < held; j += 64) differ |= pr < 0 || a.table[(size_t)it.row * a.width + j] != a.table[(size_t)pr * a.width + j];
-    if (__any(differ) && lane == 0) atomicOr(a.status, (int)ORC_KV_NOT_SHARED);
-  }
-  const int tiles = (lim - a.prefix + KT - 1) / KT;
-  int per = (tiles + a.ss - 1) / a.ss;
-  per = (per < 4 ? 4 : per) * KT;   // at least a tile for each wave
-  it.k_lo = a.prefix + sx * per;
-  it.k_hi = it.k_lo + per < lim ? it.k_lo + per : lim;
-  it.part = a.sp + sx;
-  it.f0 = i * a.group + gt * 16;
-  it.cols = a.group - gt * 16;
-  if (it.cols > 16) it.cols = 16;
-  keys_item<T, HD, NID>(a, it, room, ids, sm);
+  keys_items<T, HD, NID>(a, it, room, ids, sm);
 }
 
 // One wave per (query, head): lane s holds the weight of part s; then the lanes hold the head's dims, 16 bytes each, and a wave reads 64 * 4 / HD
