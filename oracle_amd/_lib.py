@@ -69,14 +69,14 @@ SYMBOLS = {
     'orc_decode_stream_bytes': (_L, [_P, _I]),
     'orc_decode_weight_stats': (_I, [_P, C.POINTER(_L)]),
     'orc_attn_plan': (_I, [_P, _I, _P, _I]),
-    'orc_attention_packed': (_I, [_P, _P, _P, _P, C.POINTER(_L), _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    'orc_attention_packed': (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     'orc_kv_reserve': (_I, [C.POINTER(OrcKvPages), _P, _P, _I, _P, _I, _P]),
-    'orc_kv_append': (_I, [C.POINTER(OrcKvPages), _I, _P, _I, _P, _P, C.POINTER(_L), _P]),
+    'orc_kv_append': (_I, [C.POINTER(OrcKvPages), _I, _P, _I, _P, _P, _P, _P]),
     'orc_kv_fork': (_I, [C.POINTER(OrcKvPages), _P, _P, _I, _I, _I, _P]),
     'orc_kv_free': (_I, [C.POINTER(OrcKvPages), _P, _I, _P]),
     'orc_kv_compact': (_I, [C.POINTER(OrcKvPages), C.POINTER(OrcKvPages), _P]),
     'orc_kv_attend_ws': (_L, [C.POINTER(OrcKvPages), _I, _I, _I]),
-    'orc_kv_attend': (_I, [C.POINTER(OrcKvPages), _I, _P, _P, C.POINTER(_L), _P, _P, _I, _I, _I, _F, _P, _P]),
+    'orc_kv_attend': (_I, [C.POINTER(OrcKvPages), _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P, _P]),
 }
 
 

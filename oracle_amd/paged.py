@@ -3,6 +3,8 @@ pages taken and filled (`reserve`, `append`), shared and copied (`fork`, `copy`)
 decode attention that reads a prefix shared by the whole batch once (`attend`). The C entry points are orc_attention_packed and
 orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it. There are no gradients."""
 import ctypes as C
+import functools
+import struct
 
 import torch
 
@@ -14,14 +16,15 @@ _ERRORS = ((1, 'a row outside the table'), (2, 'a row named twice (or a fork ont
            (64, 'a page outside the pool'), (128, 'rows that do not share the prefix they were attended with'))
 
 
-_I64x4, _I64x8 = C.c_int64 * 4, C.c_int64 * 8
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# strides as the C entries read them (an array of c_int64 takes four times as long to make)
+_I64x4, _I64x8 = struct.Struct('4q').pack, struct.Struct('8q').pack
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _run(device, name, *args):
     """The C entry `name` with args and the current stream of `device`, with `device` the current one."""
     fn, i = getattr(_lib.lib(), name), device.index
-    if torch.cuda.current_device() == i:
+    if _current() == i:
         rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(i):
@@ -31,6 +34,8 @@ def _run(device, name, *args):
 
 
 def _chk(t, name, dim, dtype=None, device=None):
+    if device is not None and type(t) is torch.Tensor and t.get_device() == device.index and t.dtype is dtype and t.dim() == dim and not t.requires_grad:
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f'{name} must be a CUDA tensor')
     if t.dim() != dim:
@@ -137,7 +142,7 @@ def packed_attention(q, k, v, plan, scale=None, out=None):
         raise ValueError(f'scale must be positive and finite, got {scale}')
     out = _out(out, q)
     if out is None:
-        out = (torch.empty if plan.total == tokens else torch.zeros)((tokens, hq, hd), dtype=dtype, device=device)
+        out = (torch.empty_like if plan.total == tokens else torch.zeros_like)(q, memory_format=torch.contiguous_format)
     qt, qh, qp = _place(q, 'q')
     kt, kh, kp = _place(k, 'k')
     vt, vh, vp = _place(v, 'v')
@@ -194,7 +199,15 @@ class KvPages:
         self._work = torch.zeros(8 + 4 * n_pages, dtype=torch.int32, device=kv.device)
         self._c = _lib.OrcKvPages(*[t.data_ptr() for t in (kv, table, lens, refs, self.status, self._work)], layers, n_pages, hkv, page, hd,
                                   table.shape[0], table.shape[1], _DTYPES[kv.dtype])
-        self._ref = C.byref(self._c)
+        self._ref = ref = C.byref(self._c)
+
+        @functools.lru_cache(256)
+        def attend_ws(n, hq, prefix):      # (no self in it, so no cycle keeps the pool)
+            size = _lib.lib().orc_kv_attend_ws(ref, n, hq, prefix)
+            if size < 0:
+                _lib.check(-1, 'orc_kv_attend_ws')
+            return size
+        self._attend_ws = attend_ws
 
     def _call(self, name, *args):
         _run(self.device, name, self._ref, *args)
@@ -225,7 +238,7 @@ class KvPages:
             total = n
         if not 0 <= total <= 1 << 20:
             raise ValueError(f'total must be 0..2^20, got {total}')
-        slots = torch.empty(total, dtype=torch.int32, device=self.device)
+        slots = rows.new_empty(int(total))
         self._call('orc_kv_reserve', r, c, n, slots.data_ptr(), int(total))
         return slots
 
@@ -293,11 +306,9 @@ class KvPages:
             raise ValueError(f'scale must be positive and finite, got {scale}')
         out = _out(out, q)
         if out is None:
-            out = torch.empty((n, hq, hd), dtype=self.dtype, device=self.device)
-        size = _lib.lib().orc_kv_attend_ws(self._ref, n, hq, int(prefix_tokens))
-        if size < 0:
-            _lib.check(-1, 'orc_kv_attend_ws')
-        ws = torch.empty(size // 4, dtype=torch.float32, device=self.device) if size else None
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        size = self._attend_ws(n, hq, int(prefix_tokens))
+        ws = q.new_empty(size >> 1) if size else None
         (qt, qh, qp), (ot, oh, op) = _place(q, 'q'), _place(out, 'out')
         self._call('orc_kv_attend', int(layer), qp, op, _I64x4(qt, qh, ot, oh), r, lim, n, hq, int(prefix_tokens), scale, ws.data_ptr() if size else None)
         return out
