@@ -254,8 +254,10 @@ __device__ __forceinline__ void flash_loop(Flash32<T, HD>& f, Src& src, const Im
   auto finish = [&](int t, f32x16 (&s)[2], auto par) {
     constexpr int PAR = decltype(par)::value;
     arrive();
-    src.next(t);
-    fetch(t, par);
+    if (t + 1 < tiles) {
+      src.next(t);
+      fetch(t, par);
+    }
     src.mask_last(t, s);
     f.add(PAR ? im.v1 : im.v0, s, c);
   };
@@ -267,7 +269,8 @@ __device__ __forceinline__ void flash_loop(Flash32<T, HD>& f, Src& src, const Im
   for (int r = 0; r < RND; ++r) src.V(0, r, im.v0);
 #pragma unroll
   for (int r = 0; r < RND; ++r) src.K(1, r, im.k1);
-  arrive();
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * RND) : "memory");   // the first keys (and queries): the scores need no more
+  __syncthreads();
   int t = 0;
   if (mine > 0) {
     f32x16 s[2] = {f.scores(im.k0, 0), f.scores(im.k0, 1)}, n[2];
@@ -285,6 +288,7 @@ __device__ __forceinline__ void flash_loop(Flash32<T, HD>& f, Src& src, const Im
   }
   for (t = mine; t < tiles; ++t) {   // the other waves' tiles
     arrive();
+    if (t + 1 == tiles) break;
     src.next(t);
     if (t & 1) fetch(t, odd());
     else fetch(t, even());
