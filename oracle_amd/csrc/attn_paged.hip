@@ -469,9 +469,11 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   s.sp = 0;
   if (prefix) {
     const int64_t base = (int64_t)c->n_kv_heads * s.mt;
-    // cols_item runs two to a CU: 384 items leave every fourth place to the rows' own tokens, which are bound by memory (96 rows, 4 heads a
-    // K/V head, 32k + 570 tokens: 264 items 131 us, 384 136, 504 143; without own tokens 96, 86, 87). keys_item: 512, of 256 keys and more.
-    int64_t sp = ((s.cols ? 384 : 512) + base - 1) / base;
+    // cols_item runs two to a CU: 256 items leave every other place to the rows' own tokens, which are bound by memory, not by the matrix cores
+    // (us with 256 / 384 / 512 items: 96 rows, 32 heads on 8, 32k shared + 0..2000 own tokens 117 / 127 / 134, + 200 94 / 88 / 95, without own
+    // tokens 89 / 82 / 81; 64 rows over 8k + 0..500 31 / 35 / 39; 128 rows, 16 heads on 2, 16k + 0..1000 39 / 44 / 50).
+    // keys_item: 512, of 256 keys and more.
+    int64_t sp = ((s.cols ? 256 : 512) + base - 1) / base;
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
     sp = sp < 1 ? 1 : sp > 40 ? 40 : sp;
