@@ -4,9 +4,9 @@
 // maximum m and sum of one pass over the keys (flash32.h). One workgroup = 4 waves x 32 query rows of one head.
 //
 // Long prompts are bound by the matrix cores and the softmax beside them, at the clock that the power limit leaves (about 1.75 GHz): 2 prompts of 15k
-// and 24k tokens, 32 heads on 8, head dim 128, 5.67 ms = 1157 TFLOP/s, 0.9 of an 8192^3 bf16 product on the same card. Short ones by what a tile costs
-// before its first product (Q, then two K images from HBM) and by the uneven end: 8 prompts of 640..900, 32 heads, 64 us (600 TFLOP/s,
-// 3.1 TB/s); 48 of 0..2304, 16 heads on 4, head dim 64, fp16, 159 us (710 TFLOP/s: half the products to a tile's exponentials).
+// and 24k tokens, 32 heads on 8, head dim 128, 5.55 ms = 1183 TFLOP/s, 0.92 of an 8192^3 bf16 product on the same card. Short ones by what a tile costs
+// before its first product (Q, then two K images from HBM) and by the uneven end: 8 prompts of 640..900, 32 heads, 63 us (610 TFLOP/s,
+// 3.2 TB/s); 48 of 0..2304, 16 heads on 4, head dim 64, fp16, 156 us (720 TFLOP/s: half the products to a tile's exponentials).
 // 128 rows a workgroup and not 256: those halve the reads of K / V, which L2 serves anyway, and leave fewer tiles to spread (measured slower).
 // Two workgroups fit a CU at head dim 128 (256 registers a lane), three at 64 (168).
 #include <algorithm>

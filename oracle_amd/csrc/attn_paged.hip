@@ -13,7 +13,7 @@
 //              shared and up to 300 own tokens, 66 MB in 18.5 us = 3.6 TB/s (with hardly a byte to read: 7 us).
 //   cols_item  many columns over the prefix: every wave has 32 columns of its own, 64-key tiles go through a 2-deep LDS ring that
 //              the waves share (flash32.h). Bound by the matrix cores and the softmax between the two products, then by the rows' own tokens: 96 rows of 32
-//              heads on 8, 32k shared and up to 2000 own tokens, 112 us = 470 TFLOP/s and 3.2 TB/s at once (the prefix's items first: own
+//              heads on 8, 32k shared and up to 2000 own tokens, 103 us = 510 TFLOP/s and 3.5 TB/s at once (the prefix's items first: own
 //              ones put first or between them were up to twice as slow, the workgroups being dealt out in turn).
 // The page ids of an item's keys are gathered into LDS first, so that the loop's addresses wait for no dependent load.
 #include <type_traits>
