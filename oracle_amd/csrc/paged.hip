@@ -88,13 +88,19 @@ __device__ __forceinline__ int entry_of(const int* first, int n, int x) {
 
 __device__ __forceinline__ int pages_of(const Pages& p, int tokens) { return (tokens + p.ps - 1) >> p.log_ps; }
 
-// Whether a list of rows names rows of the table, each once. seen: a bit per row (max_rows <= 65536), cleared here.
-__device__ int check_rows(const Pages& p, const int* rows, int n, unsigned* seen) {
+// Entry t of a list of rows, and the tokens of that row (0 where it is outside the table; 0 and 0 behind the list). The loads are asked for before the rows
+// are checked: their latency is most of what these kernels take.
+__device__ __forceinline__ int row_of(const int* rows, int n) { return (int)threadIdx.x < n ? rows[threadIdx.x] : 0; }
+__device__ __forceinline__ int tokens_of(const Pages& p, int r, int n) {
+  const int len = p.lens[r >= 0 && r < p.max_rows ? r : 0];
+  return (int)threadIdx.x < n && r >= 0 && r < p.max_rows ? len : 0;
+}
+// Whether the threads' rows are rows of the table, each once. seen: a bit per row (max_rows <= 65536), cleared here.
+__device__ int check_rows(const Pages& p, int r, int n, unsigned* seen) {
   for (int i = threadIdx.x; i < (p.max_rows + 31) / 32; i += NT) seen[i] = 0;
   __syncthreads();
   int bad = 0;
   if ((int)threadIdx.x < n) {
-    const int r = rows[threadIdx.x];
     if (r < 0 || r >= p.max_rows) bad = ORC_KV_BAD_ROW;
     else if (atomicOr(&seen[r >> 5], 1u << (r & 31)) >> (r & 31) & 1) bad = ORC_KV_ROW_TWICE;
   }
@@ -118,12 +124,10 @@ __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, c
   __shared__ unsigned seen[2048];
   __shared__ int tok0[NT], page0[NT], from[NT], of[NT];   // of every list entry: first new token, first new page, tokens held before, row
   const int t = threadIdx.x;
-  int bad = check_rows(p, rows, n, seen);
-  int r = 0, old = 0, add = 0;
+  const int r = row_of(rows, n), more = counts ? row_of(counts, n) : 1, old = tokens_of(p, r, n);
+  int bad = check_rows(p, r, n, seen), add = 0;
   if (t < n && !bad) {
-    r = rows[t];
-    old = p.lens[r];
-    add = counts ? counts[t] : 1;
+    add = more;
     if (add < 0 || add > total) bad = ORC_KV_BAD_COUNT;   // (more than `total` fails below anyway; here it bounds the sums)
     else if (old < 0 || (long)old + add > (long)p.width * p.ps) bad = ORC_KV_ROW_FULL;
     if (bad) add = 0;
@@ -185,17 +189,15 @@ __global__ __launch_bounds__(NT) void fork_kernel(Pages p, const int* src, const
   __shared__ int src_of[NT], dst_of[NT], len_of[NT], page0[NT], most_sh;   // of every pair; page0: its first fresh page
   const int t = threadIdx.x;
   if (t == 0) most_sh = 0;
-  int bad = check_rows(p, dst, n, seen);
+  const int d = row_of(dst, n), s = row_of(src, n), held = tokens_of(p, d, n), source = tokens_of(p, s, n);
+  int bad = check_rows(p, d, n, seen), len = 0;
   __syncthreads();
-  int s = 0, d = 0, len = 0;
   if (t < n && !bad) {
-    s = src[t];
-    d = dst[t];
     if (s < 0 || s >= p.max_rows) bad = ORC_KV_BAD_ROW;
     else if (seen[s >> 5] >> (s & 31) & 1) bad = ORC_KV_ROW_TWICE;   // a source that is also a destination
-    else if (p.lens[d] != 0) bad = ORC_KV_NOT_EMPTY;
+    else if (held != 0) bad = ORC_KV_NOT_EMPTY;
     else {
-      len = p.lens[s];
+      len = source;
       if (n_tokens >= 0 && n_tokens < len) len = n_tokens;
       if (len < 0 || len > p.width * p.ps) { bad = ORC_KV_BAD_COUNT; len = 0; }
     }
@@ -268,34 +270,32 @@ __global__ __launch_bounds__(256) void copy_kernel(const char* from, char* to, c
 __global__ __launch_bounds__(NT) void free_kernel(Pages p, const int* rows, int n) {
   __shared__ int sh[NT / 64 + 1];
   __shared__ unsigned seen[2048];
-  __shared__ int pages[NT], most_sh;
+  __shared__ int pages[NT], of[NT], most_sh;   // of every row: its pages, its place in the table
   const int t = threadIdx.x;
   if (t == 0) most_sh = 0;
-  int bad = check_rows(p, rows, n, seen);
+  const int r = row_of(rows, n), len = tokens_of(p, r, n);
+  int bad = check_rows(p, r, n, seen);
   bad = block_or(bad, sh);
   if (bad) {
     if (t == 0) atomicOr(p.status, bad);
     return;
   }
-  // Up to the longest row, not the table's width (64 rows of 13 pages in a table 4096 wide: 108 -> 7 us; of 2000: 186 -> 51; 16 of 13 in 16: 6.2 -> 6.7).
-  int used = 0;   // the row's pages
-  if (t < n) {
-    const int len = p.lens[rows[t]];
-    used = len <= 0 ? 0 : len < p.width * p.ps ? pages_of(p, len) : p.width;
-    if (used) atomicMax(&most_sh, used);
-  }
+  // Up to the longest row, not the table's width (64 rows of 13 pages in a table 4096 wide: 108 -> 7 us; of 2000: 186 -> 39; 16 of 13 in 16: 6.2 -> 6.6).
+  const int used = len <= 0 ? 0 : len < p.width * p.ps ? pages_of(p, len) : p.width;
+  if (used) atomicMax(&most_sh, used);
   pages[t] = used;
+  of[t] = r;
   __syncthreads();
   const int most = most_sh;
   for (int x = t; x < n * most; x += NT) {
     const int i = x / most, j = x - i * most;
     if (j >= pages[i]) continue;
-    int* e = &p.table[(size_t)rows[i] * p.width + j];
+    int* e = &p.table[(size_t)of[i] * p.width + j];
     const int page = *e;
     if (page >= 0 && page < p.n_pages) atomicSub(&p.refs[page], 1);
     *e = -1;
   }
-  if (t < n) p.lens[rows[t]] = 0;
+  if (t < n) p.lens[r] = 0;
 }
 
 // where every held page goes: map[page] (work list 3) and the copies; in place only pages behind the last to keep move
