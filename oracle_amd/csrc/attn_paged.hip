@@ -27,7 +27,8 @@ namespace {
 constexpr int KT = 32;            // keys of a wave's tile in keys_item
 constexpr int IDS = 512;          // page ids held in LDS at a time by keys_item
 constexpr int IDS_COLS = 2048;    // by cols_item, whose range has to fit
-constexpr int MAX_PARTS = 64;     // parts of one query (a lane of the combining wave each)
+constexpr int MAX_SP = 40, MAX_SS = 16;   // parts of a query, of the prefix and of its row's own tokens
+static_assert(MAX_SP + MAX_SS <= 64, "a lane of the combining wave each");
 
 struct AttendArgs {
   const char *k, *v;              // this layer's K / V pages
@@ -459,10 +460,10 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   // columns is cheap while the first one's pages are in the caches (keys / cols us at 32 columns: 32 K/V heads, 768 shared tokens 18.3 / 20.8, 4k
   // 28.2 / 30.6; 2 heads, 16k 17.4 / 20.9) and is not beyond (32 heads, 8k, 134 MB 42.9 / 43.2; 16k 71.9 / 66.0); more passes cost more (48
   // columns: 8 heads, 4k 15.3 / 15.6, 32k 52.2 / 39.1; 32 heads, 8k 60.3 / 51.1).
-  // cols_item reads at most IDS_COLS - 4 pages, of 40 parts at the most.
+  // cols_item reads at most IDS_COLS - 4 pages, of MAX_SP parts at the most.
   const int64_t range = (int64_t)(IDS_COLS - 4) * c->page_size, least_sp = (prefix + range - 1) / range;
   const int64_t bytes = (int64_t)prefix * c->n_kv_heads * c->head_dim * 4;
-  s.cols = cols > (bytes > 128 << 20 ? 16 : 32) && least_sp <= 40;
+  s.cols = cols > (bytes > 128 << 20 ? 16 : 32) && least_sp <= MAX_SP;
   const int wide = s.cols ? 128 : 16;
   s.mt = prefix ? (int)((cols + wide - 1) / wide) : 0;
   s.gt = (group + 15) / 16;
@@ -476,7 +477,7 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
     int64_t sp = ((s.cols ? 256 : 512) + base - 1) / base;
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
-    sp = sp < 1 ? 1 : sp > 40 ? 40 : sp;
+    sp = sp < 1 ? 1 : sp > MAX_SP ? MAX_SP : sp;
     s.sp = (int)(s.cols && sp < least_sp ? least_sp : sp);
   }
   const int64_t own = (int64_t)n * c->n_kv_heads * s.gt;
@@ -484,7 +485,7 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   int64_t ss = (512 + own - 1) / own;
   const int64_t most_ss = (left + 255) / 256;
   ss = ss < most_ss ? ss : most_ss;
-  s.ss = (int)(ss < 1 ? 1 : ss > 16 ? 16 : ss);
+  s.ss = (int)(ss < 1 ? 1 : ss > MAX_SS ? MAX_SS : ss);
   return s;
 }
 
