@@ -244,11 +244,14 @@ __device__ __forceinline__ bool keys_item(const AttendArgs& a, const Item& it, c
 }
 
 // The item's columns, 16 at a time; where a value that not all of them see is infinite or NaN, again one by one, up to the column's last token.
+// A barrier in front of every pass but the first: its waves write sm and the rooms, which the pass before still joins (with one column by a single
+// wave), and a pass whose column ends in front of the item has no load_ids to wait in.
 template <typename T, int HD, int NID>
 __device__ __forceinline__ void keys_items(const AttendArgs& a, const Item& it, const Rooms& room, int* ids, float* sm) {
   Item sub = it;
   int x = 0, wide = 16, back = 0;
-  while (x < it.cols) {
+  for (bool first = true; x < it.cols; first = false) {
+    if (!first) __syncthreads();
     sub.f0 = it.f0 + x;
     sub.cols = it.cols - x < wide ? it.cols - x : wide;
     sub.k_hi = it.k_hi;
