@@ -198,7 +198,8 @@ int orc_decode_weight_stats(orc_engine* e, int64_t* out6);
  * the number of tiles (out_host may be NULL to count them), -1 on error.
  * orc_attention_packed: causal attention inside every sequence, token t of a sequence over its tokens 0..t.
  * q (total, n_heads, head_dim), k / v (total, n_kv_heads, head_dim), out like q; strides8 = {q token, q head, k token, k head,
- * v token, v head, out token, out head}; work = the plan on the device; n_work * n_heads < 2^24. Rows of `out` that no sequence covers are left as they are; `out` may be q. */
+ * v token, v head, out token, out head}; work = the plan on the device; n_work * n_heads < 2^24. Rows of `out` that no sequence covers are left as they are. `out` may be q
+ * itself; an `out` that lies over q in another way, or over k or v, is refused (views of one memory with different token strides are taken to overlap). */
 int orc_attn_plan(const int32_t* lens_host, int n, int32_t* out_host, int capacity);
 int orc_attention_packed(const void* q, const void* k, const void* v, void* out, const int64_t* strides8, const int32_t* work, int n_work,
                          int total, int n_heads, int n_kv_heads, int head_dim, int dtype, float scale, void* stream);
@@ -236,7 +237,8 @@ int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, void* stream
  * the first limits[i] tokens (NULL: all lens[rows[i]]) of row rows[i]. The first prefix_tokens (a multiple of page_size) are held
  * on the same pages by every named row and are read once for all of them, through rows[0]; rows that do not share them set
  * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros. Tokens on a page outside the pool are not attended.
- * What lies behind a query's tokens has no influence, infinities and NaN included. `out` may be q.
+ * What lies behind a query's tokens has no influence, infinities and NaN included. `out` may be q itself, and lies neither
+ * over q in another way nor over the pool.
  * ws: orc_kv_attend_ws bytes of scratch, 16-byte aligned. */
 int64_t orc_kv_attend_ws(const orc_kv_pages* c, int n, int n_heads, int prefix_tokens);
 int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, void* out, const int64_t* strides4, const int32_t* rows, const int32_t* limits,

@@ -10,6 +10,7 @@
 // 128 rows a workgroup and not 256: those halve the reads of K / V, which L2 serves anyway, and leave fewer tiles to spread (measured slower).
 // Two workgroups fit a CU at head dim 128 (256 registers a lane), three at 64 (168).
 #include <algorithm>
+#include <cstdlib>
 
 #include "../../include/oracle_hip.h"
 #include "kernels.h"
@@ -160,6 +161,46 @@ __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a, int4* work) {
 
 }  // namespace
 
+bool views_meet(HeadView a, HeadView b) {
+  for (HeadView* x : {&a, &b}) {
+    if (x->tokens < 1) return false;
+    if (x->tokens == 1) x->ts = 0;   // the stride of one element does not matter
+    if (x->heads == 1) x->hs = 0;
+  }
+  const int64_t d0 = ((intptr_t)b.p - (intptr_t)a.p) / 2;   // both start on 16 bytes
+  const int64_t end_a = (a.tokens - 1) * a.ts + (a.heads - 1) * a.hs + a.hd, end_b = (b.tokens - 1) * b.ts + (b.heads - 1) * b.hs + b.hd;
+  if (d0 >= end_a || -d0 >= end_b) return false;
+  if (a.tokens > 1 && b.tokens > 1 && a.ts != b.ts) return true;
+  const int64_t ts = a.tokens > 1 ? a.ts : b.ts, row_a = (a.heads - 1) * a.hs + a.hd, row_b = (b.heads - 1) * b.hs + b.hd;
+  if (ts > 0) {   // slices of one projection's rows: b's part of a row behind a's
+    const int64_t at = (d0 % ts + ts) % ts;
+    if (at >= row_a && at + row_b <= ts) return false;
+  }
+  // heads d apart, tokens k apart: closest for the two k around -d / ts
+  auto close = [&](int64_t d) {
+    const int64_t lo = -(a.tokens - 1), hi = b.tokens - 1, k0 = ts > 0 ? -d / ts : 0;
+    for (int64_t k = k0 - 1; k <= k0 + 1; ++k)
+      if (std::abs(d + std::min(std::max(k, lo), hi) * ts) < std::max(a.hd, b.hd)) return true;
+    return false;
+  };
+  const bool same = a.hs == b.hs || a.heads == 1 || b.heads == 1;
+  const int64_t hs = a.heads > 1 ? a.hs : b.hs;
+  if (same) {
+    for (int64_t h = -(int64_t)(a.heads - 1); h < b.heads; ++h)
+      if (close(d0 + h * hs)) return true;
+    return false;
+  }
+  for (int64_t x = 0; x < a.heads; ++x)
+    for (int64_t y = 0; y < b.heads; ++y)
+      if (close(d0 + y * b.hs - x * a.hs)) return true;
+  return false;
+}
+
+bool out_meets_q(const HeadView& o, const HeadView& q) {
+  if (o.p == q.p && (o.tokens <= 1 || o.ts == q.ts) && (o.heads == 1 || o.hs == q.hs)) return false;
+  return views_meet(o, q);
+}
+
 int attn_plan_ints(int rows) { return (rows / ROWS + kMaxRows) * 4; }
 
 int launch_attn_plan(const PackedRows& p, int32_t* work, hipStream_t s) {
@@ -224,6 +265,10 @@ extern "C" int orc_attention_packed(const void* q, const void* k, const void* v,
   if (n_work == 0) return 0;
   if (!q || !k || !v || !out || !work) return orc_fail(who, "null argument");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)work) & 15) return orc_fail(who, "tensors are not aligned to 16 bytes");
+  const HeadView vo{out, st[6], st[7], total, n_heads, head_dim};
+  if (views_meet(vo, {k, st[2], st[3], total, n_kv_heads, head_dim}) || views_meet(vo, {v, st[4], st[5], total, n_kv_heads, head_dim}))
+    return orc_fail(who, "out lies over k or v");
+  if (out_meets_q(vo, {q, st[0], st[1], total, n_heads, head_dim})) return orc_fail(who, "out lies over q and is not q");
   PackedArgs a;
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (char*)out;
   a.q_ts = st[0]; a.q_hs = st[1]; a.k_ts = st[2]; a.k_hs = st[3]; a.v_ts = st[4]; a.v_hs = st[5]; a.o_ts = st[6]; a.o_hs = st[7];

@@ -540,8 +540,13 @@ extern "C" int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, vo
   const Split s = split_of(c, n, n_heads, prefix);
   if (!q || !out || !rows || !c->kv || !c->table || !c->lens || !c->status || (s.sp + s.ss > 1 && !ws)) return orc_fail(who, "null argument");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)c->kv | (uintptr_t)ws) & 15) return orc_fail(who, "tensors are not aligned to 16 bytes");
+  const HeadView vo{out, st[2], st[3], n, n_heads, c->head_dim};
+  if (out_meets_q(vo, {q, st[0], st[1], n, n_heads, c->head_dim})) return orc_fail(who, "out lies over q and is not q");
   AttendArgs a;
   const size_t page = (size_t)c->n_kv_heads * c->page_size * c->head_dim;
+  const char* kv_end = (const char*)c->kv + (size_t)c->n_layers * 2 * c->n_pages * page * 2;
+  if ((const char*)out < kv_end && (const char*)out + ((n - 1) * vo.ts + (n_heads - 1) * vo.hs + c->head_dim) * 2 > (const char*)c->kv)
+    return orc_fail(who, "out lies over the pool");
   a.k = (const char*)c->kv + (size_t)layer * 2 * c->n_pages * page * 2;
   a.v = a.k + (size_t)c->n_pages * page * 2;
   a.page_elems = (long)page;

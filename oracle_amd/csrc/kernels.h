@@ -25,6 +25,13 @@ struct PackedRows {
   RowMap map;
 };
 
+// (tokens, heads, hd) 16-bit values at p, strides in elements. views_meet: whether an element of one may be one of the other's; exact where the token
+// strides are the same (slices of one tensor), else by the memory they span.
+struct HeadView { const void* p; int64_t ts, hs; int64_t tokens; int heads, hd; };
+bool views_meet(HeadView a, HeadView b);
+// out may be q itself, element for element, and must not meet it otherwise
+bool out_meets_q(const HeadView& out, const HeadView& q);
+
 enum { EPI_NONE = 0, EPI_QUICKGELU = 1, EPI_GELU = 2, EPI_RESIDUAL = 3, EPI_SWIGLU = 4, EPI_F32 = 5, EPI_ROPE_KV = 6 };
 
 struct GemmArgs {

@@ -121,7 +121,7 @@ class PackedPlan:
 def packed_attention(q, k, v, plan, scale=None, out=None):
     """Causal attention inside every prompt of `plan`: q (T, Hq, hd), k / v (T, Hkv, hd) with T >= plan.total, hd 64 or 128, Hq a multiple of
     Hkv; slices of a fused projection are taken as they are. scale defaults to hd ** -0.5. Rows of `out` behind the last prompt are left
-    as they are (zero in a tensor made here). `out` may be q, but must not lie over k or v."""
+    as they are (zero in a tensor made here). `out` may be q; one that lies over q in another way, or over k or v, is refused."""
     _chk(q, 'q', 3)
     dtype, device = q.dtype, q.device
     _chk(k, 'k', 3, dtype, device)
@@ -289,7 +289,8 @@ class KvPages:
         """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
         n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
         once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
-        gives zeros; what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q."""
+        gives zeros; what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in another way, or over
+        the pool, is refused."""
         _chk(q, 'q', 3, self.dtype, self.device)
         n, hq, hd = q.shape
         if hd != self.head_dim:

@@ -3,8 +3,9 @@ are test_paged_gpu's."""
 import pytest
 import torch
 
-from oracle_amd.paged import KvPages
-from test_paged_gpu import attention64, close, filled, ints
+from oracle_amd._lib import OracleHipError
+from oracle_amd.paged import PackedPlan, packed_attention
+from test_paged_gpu import attention64, close, filled, ints, qkv
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -36,3 +37,37 @@ def test_attend_columns_without_keys_behind_columns_with_keys(n, hq, hkv, hd, dt
                 keep = [d for d in range(hd) if d != 7 or m <= 200]       # `dense` was taken before the NaN went in
                 close(first[i][:, keep], ref[:, keep], tol[:, keep], (most, i))
                 assert 7 in keep or first[i, :, 7].isnan().all()
+
+
+def test_packed_attention_into_slices_of_the_projection():
+    lens, hq, hkv, hd = [90, 33], 4, 4, 64
+    q, k, v = qkv(sum(lens), hq, hkv, hd, FP, 90)
+    plan = PackedPlan(lens)
+    want = packed_attention(q, k, v, plan)
+    rows = torch.cat([q, k, v], 1)                                                   # (T, heads of q, k, v, hd)
+    kv = rows[:, hq:].clone()
+    out = rows[:, :hq]
+    assert packed_attention(out, rows[:, hq:2 * hq], rows[:, 2 * hq:], plan, out=out) is out
+    assert torch.equal(out, want) and torch.equal(rows[:, hq:], kv)
+    heads = torch.stack([q, k, v], 2)                                                # (T, heads, q k v, hd)
+    out = heads[:, :, 0]
+    assert packed_attention(out, heads[:, :, 1], heads[:, :, 2], plan, out=out) is out
+    assert torch.equal(out, want) and torch.equal(heads[:, :, 1], k)
+    rows = torch.cat([q, k, v], 1)
+    for out, text in ((rows[:, hq:2 * hq], 'k or v'), (rows[:, 2 * hq:], 'k or v'), (rows[:, 1:1 + hq], 'k or v')):
+        with pytest.raises(OracleHipError, match=text):
+            packed_attention(rows[:, :hq], rows[:, hq:2 * hq], rows[:, 2 * hq:], plan, out=out)
+    room = torch.zeros(sum(lens) + 1, hq, hd, dtype=FP, device=DEV)
+    with pytest.raises(OracleHipError, match='over q'):
+        packed_attention(room[1:], k, v, plan, out=room[:-1])
+
+
+def test_attend_into_the_pool_or_a_shifted_query_is_refused():
+    c, _ = filled(3, 0, [5, 70, 2], 64, 2, 64, FP, 91)
+    rows, room = ints([0, 1, 2]), torch.zeros(4, 4, 64, dtype=FP, device=DEV)
+    with pytest.raises(OracleHipError, match='over q'):
+        c.attend(1, room[1:], rows, out=room[:-1])
+    before = c.kv.clone()
+    with pytest.raises(OracleHipError, match='over the pool'):
+        c.attend(1, room[1:], rows, out=c.kv.view(-1)[:3 * 4 * 64].view(3, 4, 64))
+    assert torch.equal(c.kv.view(torch.int16), before.view(torch.int16))
