@@ -1,12 +1,14 @@
 """Prompts of different lengths in one pass, and a paged KV cache: attention over packed prompts (`packed_attention`), and `KvPages` --
 pages taken and filled (`reserve`, `append`), shared and copied (`fork`, `copy`), given back (`free`), moved together (`compact`), and
 decode attention that reads a prefix shared by the whole batch once (`attend`). The C entry points are orc_attention_packed and
-orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it. There are no gradients."""
+orc_kv_* of include/oracle_hip.h; tensors are bf16 or fp16 on one GPU, and every call runs on that GPU's current stream without waiting for it. There are no
+derivatives: tensors that want a gradient, or have a tangent, are refused."""
 import ctypes as C
 import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -49,6 +51,13 @@ def _chk(t, name, dim, dtype=None, device=None):
         raise ValueError(f'{name} is on {t.device}, not on {device}')
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{name} requires a gradient and the call has none: detach it, or call under torch.no_grad()')
+
+
+def _no_tangents(**tensors):
+    """Inside a level of forward-mode differentiation (nothing to look for outside)"""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name} has a tangent and the call has no derivative: pass forward_ad.unpack_dual({name}).primal')
 
 
 def _place(t, name):
@@ -126,6 +135,8 @@ def packed_attention(q, k, v, plan, scale=None, out=None):
     dtype, device = q.dtype, q.device
     _chk(k, 'k', 3, dtype, device)
     _chk(v, 'v', 3, dtype, device)
+    if forward_ad._current_level >= 0:
+        _no_tangents(q=q, k=k, v=v, out=out)
     (tokens, hq, hd), (k_tokens, hkv, k_hd) = q.shape, k.shape
     if k.shape != v.shape or k_tokens != tokens or k_hd != hd:
         raise ValueError(f'q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together')
@@ -181,6 +192,8 @@ class KvPages:
 
     def _adopt(self, kv, table, lens, refs):
         _chk(kv, 'kv', 6)
+        if forward_ad._current_level >= 0:
+            _no_tangents(kv=kv)
         for t, name, dim in ((table, 'table', 2), (lens, 'lens', 1), (refs, 'refs', 1)):
             _chk(t, name, dim, torch.int32, kv.device)
         if not all(t.is_contiguous() for t in (kv, table, lens, refs)) or kv.data_ptr() % 16:
@@ -246,6 +259,8 @@ class KvPages:
         """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`, each named once; a place of -1 is skipped."""
         _chk(k, 'k', 3, self.dtype, self.device)
         _chk(v, 'v', 3, self.dtype, self.device)
+        if forward_ad._current_level >= 0:
+            _no_tangents(k=k, v=v)
         s = _ints(slots, 'slots', self.device)
         want = (slots.numel(), self.n_kv_heads, self.head_dim)
         if k.shape != want or v.shape != want:
@@ -292,6 +307,8 @@ class KvPages:
         gives zeros; what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in another way, or over
         the pool, is refused."""
         _chk(q, 'q', 3, self.dtype, self.device)
+        if forward_ad._current_level >= 0:
+            _no_tangents(q=q, out=out)
         n, hq, hd = q.shape
         if hd != self.head_dim:
             raise ValueError(f'head_dim of q is {hd}, of the cache {self.head_dim}')

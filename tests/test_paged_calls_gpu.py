@@ -2,9 +2,10 @@
 are test_paged_gpu's."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle_amd._lib import OracleHipError
-from oracle_amd.paged import PackedPlan, packed_attention
+from oracle_amd.paged import KvPages, PackedPlan, packed_attention
 from test_paged_gpu import attention64, close, filled, ints, qkv
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +72,27 @@ def test_attend_into_the_pool_or_a_shifted_query_is_refused():
     with pytest.raises(OracleHipError, match='over the pool'):
         c.attend(1, room[1:], rows, out=c.kv.view(-1)[:3 * 4 * 64].view(3, 4, 64))
     assert torch.equal(c.kv.view(torch.int16), before.view(torch.int16))
+
+
+def test_tensors_with_a_tangent_are_refused():
+    c, _ = filled(2, 0, [3, 4], 32, 2, 64, FP, 92)
+    q, k, v = qkv(16, 4, 2, 64, FP, 92)
+    plan, rows = PackedPlan([16]), ints([0, 1])
+    slots = c.reserve(rows)
+    c.append(1, slots, k[:2], v[:2])                  # (what `filled` leaves in a free place is NaN)
+    want, one = packed_attention(q, k, v, plan), c.attend(1, q[:2], rows)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))      # noqa: E731
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = dual(x[i])
+            for mode in (torch.enable_grad(), torch.no_grad()):
+                with mode, pytest.raises(ValueError, match='tangent'):
+                    packed_attention(*x, plan)
+        for call in (lambda: packed_attention(q, k, v, plan, out=dual(torch.empty_like(q))), lambda: c.attend(1, dual(q[:2]), rows),
+                     lambda: c.attend(1, q[:2], rows, out=dual(torch.empty_like(q[:2]))), lambda: c.append(1, slots, dual(k[:2]), v[:2]),
+                     lambda: c.append(1, slots, k[:2], dual(v[:2])), lambda: KvPages.wrap(dual(c.kv), c.table, c.lens, c.refs)):
+            with pytest.raises(ValueError, match='tangent'):
+                call()
+        assert torch.equal(packed_attention(forward_ad.unpack_dual(dual(q)).primal, k, v, plan), want)      # without one: as outside
+        assert torch.equal(c.attend(1, q[:2], rows), one)
