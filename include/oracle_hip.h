@@ -239,7 +239,8 @@ int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, void* stream
  * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros. Tokens on a page outside the pool are not attended.
  * What lies behind a query's tokens has no influence, infinities and NaN included. `out` may be q itself, and lies neither
  * over q in another way nor over the pool.
- * ws: orc_kv_attend_ws bytes of scratch, 16-byte aligned. */
+ * ws: orc_kv_attend_ws bytes of scratch, 16-byte aligned; -1 for a call that no launch can hold (more than 2^24 - 1 workgroups), which orc_kv_attend
+ * refuses too. */
 int64_t orc_kv_attend_ws(const orc_kv_pages* c, int n, int n_heads, int prefix_tokens);
 int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, void* out, const int64_t* strides4, const int32_t* rows, const int32_t* limits,
                   int n, int n_heads, int prefix_tokens, float scale, void* ws, void* stream);

@@ -504,8 +504,15 @@ const char* bad_call(const orc_kv_pages* c, int n, int n_heads, int prefix) {
   return nullptr;
 }
 
+// 256 threads a workgroup, 32 bits of threads a launch; cols_item counts (query, head, part) in 32 bits
+bool too_large(const orc_kv_pages* c, int n, int n_heads, const Split& s) {
+  const int64_t items = (int64_t)c->n_kv_heads * s.mt * s.sp + (int64_t)n * c->n_kv_heads * s.gt * s.ss, waves = (int64_t)n * n_heads;
+  return items > 0xffffff || (waves + 3) / 4 > 0xffffff || waves * (s.sp + s.ss) > 0x7fffffff;
+}
+constexpr const char* TOO_LARGE = "too many queries and heads: 2^24 - 1 workgroups and 2^31 - 1 parts at the most";
+
 template <typename T, int HD, bool COLS> hipError_t launch_cols(const AttendArgs& a, hipStream_t s) {
-  const unsigned grid = (unsigned)(a.hkv * a.mt * a.sp + a.n * a.hkv * a.gt * a.ss);
+  const unsigned grid = (unsigned)(a.hkv * a.mt * a.sp + a.n * a.hkv * a.gt * a.ss);   // (not too_large)
   hipLaunchKernelGGL((attend_kernel<T, HD, COLS>), dim3(grid), dim3(256), 0, s, a);
   if (a.sp + a.ss > 1)
     hipLaunchKernelGGL((combine_kernel<T, HD>), dim3((unsigned)(((int64_t)a.n * a.hq + 3) / 4)), dim3(256), 0, s, a);
@@ -521,6 +528,7 @@ extern "C" int64_t orc_kv_attend_ws(const orc_kv_pages* c, int n, int n_heads, i
   const char* bad = bad_call(c, n, n_heads, prefix);
   if (bad) return orc_fail("orc_kv_attend_ws", bad);
   const Split s = split_of(c, n < 1 ? 1 : n, n_heads, prefix);
+  if (too_large(c, n, n_heads, s)) return orc_fail("orc_kv_attend_ws", TOO_LARGE);
   return s.sp + s.ss == 1 ? 0 : (int64_t)n * n_heads * (s.sp + s.ss) * (c->head_dim + 2) * 4;
 }
 
@@ -538,6 +546,7 @@ extern "C" int orc_kv_attend(const orc_kv_pages* c, int layer, const void* q, vo
     if (st[i] < 0 || st[i] % 8) return orc_fail(who, "strides are not multiples of 8 elements");
   if (n == 0) return 0;
   const Split s = split_of(c, n, n_heads, prefix);
+  if (too_large(c, n, n_heads, s)) return orc_fail(who, TOO_LARGE);
   if (!q || !out || !rows || !c->kv || !c->table || !c->lens || !c->status || (s.sp + s.ss > 1 && !ws)) return orc_fail(who, "null argument");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)c->kv | (uintptr_t)ws) & 15) return orc_fail(who, "tensors are not aligned to 16 bytes");
   const HeadView vo{out, st[2], st[3], n, n_heads, c->head_dim};

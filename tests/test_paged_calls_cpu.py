@@ -96,3 +96,16 @@ def test_attend_refuses_an_out_over_its_queries_or_the_pool(lib):
     assert 'over q' in attend(q, q + 1024) and 'over q' in attend(q, q + 128) and 'over q' in attend(q, q, out_ts=1024)
     assert attend(q, (1 << 30) + pool) is None and attend(q, (1 << 30) - 3 * 1024) is None
     assert 'pool' in attend(q, (1 << 30) + pool - 1024) and 'pool' in attend(q, (1 << 30) - 3 * 1024 + 16)
+
+
+# items of the prefix (wide columns and 16 at a time), of the rows' own tokens, and the waves that join
+@pytest.mark.parametrize('hkv, hq, n, prefix', [(16384, 16384, 1024, 0), (16384, 16384, 1024, 64), (1, 1 << 17, 1024, 0), (1, 60000, 1024, 16 * 40 * 2044), (131072, 131072, 200, 64)])
+def test_attend_refuses_what_no_launch_can_hold(lib, hkv, hq, n, prefix):
+    fields = dict(kv=1 << 40, table=4096, lens=4096, refs=4096, status=4096, work=4096, n_layers=1, n_pages=4, n_kv_heads=hkv, page_size=16, head_dim=64,
+                  max_rows=4, max_row_pages=1 << 20, dtype=0)
+    c = _lib.OrcKvPages(*[fields[x] for x, _ in _lib.OrcKvPages._fields_])
+    assert lib.orc_kv_attend_ws(C.byref(c), n, hq, prefix) == -1 and b'too many' in lib.orc_last_error()
+    st = (C.c_int64 * 4)(hq * 64, 64, hq * 64, 64)
+    assert lib.orc_kv_attend(C.byref(c), 0, 4096, 4096, st, 4096, None, n, hq, prefix, 0.1, 4096, None) == -1
+    assert b'too many' in lib.orc_last_error()
+    assert lib.orc_kv_attend_ws(C.byref(c), 1, hkv, 0) >= 0
