@@ -219,7 +219,8 @@ typedef struct orc_kv_pages {
 enum { ORC_KV_BAD_ROW = 1, ORC_KV_ROW_TWICE = 2, ORC_KV_BAD_COUNT = 4, ORC_KV_ROW_FULL = 8, ORC_KV_POOL_FULL = 16, ORC_KV_NOT_EMPTY = 32,
        ORC_KV_BAD_PAGE = 64, ORC_KV_NOT_SHARED = 128 };
 /* counts[i] more tokens (NULL: one) for row rows[i]; slots[0..total): place (page * page_size + offset) of every new token, the rows' tokens
- * one behind the other in list order, -1 behind the last and everywhere when the call fails. */
+ * one behind the other in list order, -1 behind the last and everywhere when the call fails. A row whose begun page is outside the pool
+ * gets no more tokens (ORC_KV_BAD_PAGE). */
 int orc_kv_reserve(const orc_kv_pages* c, const int32_t* rows, const int32_t* counts, int n, int32_t* slots, int total, void* stream);
 /* K / V of `total` tokens (token and head strides in elements) into their slots of one layer; a slot outside the pool is skipped. */
 int orc_kv_append(const orc_kv_pages* c, int layer, const int32_t* slots, int total, const void* k, const void* v, const int64_t* strides4,

@@ -132,6 +132,8 @@ __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, c
     else if (old < 0 || (long)old + add > (long)p.width * p.ps) bad = ORC_KV_ROW_FULL;
     if (bad) add = 0;
   }
+  int part = 0;   // the page that the row's next token goes to, where it has been begun: looked at behind the sums, its load meanwhile in flight
+  if (add > 0 && (old & (p.ps - 1))) part = p.table[(size_t)r * p.width + (old >> p.log_ps)];
   bad = block_or(bad, sh);
   int need_all = 0, add_all = 0, at = 0, first = 0;
   if (!bad) {
@@ -141,7 +143,8 @@ __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, c
   int* list = p.work + 8;
   if (!bad) {
     at = block_scan(pages_of(p, old + add) - pages_of(p, old), &need_all, sh);
-    if (need_all > p.n_pages || !lowest_free(p, need_all, list, sh)) bad = ORC_KV_POOL_FULL;
+    if (__syncthreads_or(part < 0 || part >= p.n_pages)) bad = ORC_KV_BAD_PAGE;
+    else if (need_all > p.n_pages || !lowest_free(p, need_all, list, sh)) bad = ORC_KV_POOL_FULL;
   }
   if (bad) {   // the same for all threads
     if (t == 0) atomicOr(p.status, bad);

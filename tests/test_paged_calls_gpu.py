@@ -96,3 +96,18 @@ def test_tensors_with_a_tangent_are_refused():
                 call()
         assert torch.equal(packed_attention(forward_ad.unpack_dual(dual(q)).primal, k, v, plan), want)      # without one: as outside
         assert torch.equal(c.attend(1, q[:2], rows), one)
+
+
+# A row whose last, part page is not one of the pool's: its next tokens have no place (page * page_size may even come out as another page's)
+@pytest.mark.parametrize('bad', [-1, 40, (1 << 28) + 1, -(1 << 28)])
+def test_reserve_refuses_a_part_page_outside_the_pool(bad):
+    c, _ = filled(3, 0, [21, 5, 16], 16, 2, 64, FP, 93, extra=6)
+    c.table[0, 1] = bad
+    before = [x.clone() for x in (c.table, c.lens, c.refs)]
+    for rows, counts in ((ints([0]), None), (ints([1, 0, 2]), ints([3, 20, 1])), (ints([2, 1, 0]), ints([0, 0, 1]))):
+        slots = c.reserve(rows, counts, total=None if counts is None else 44)
+        with pytest.raises(OracleHipError, match='a page outside the pool'):
+            c.check()
+        assert (slots == -1).all() and all(torch.equal(x, y) for x, y in zip(before, (c.table, c.lens, c.refs)))
+    assert (c.reserve(ints([0, 1, 2]), ints([0, 2, 1]), total=3) >= 0).all()      # no token for that row: its page does not matter
+    c.check()
