@@ -237,7 +237,8 @@ int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, void* stream
 /* One token of attention per query over the cache: query i (q [n][n_heads][head_dim], strides4 = {q token, q head, out token, out head}) reads
  * the first limits[i] tokens (NULL: all lens[rows[i]]) of row rows[i]. The first prefix_tokens (a multiple of page_size) are held
  * on the same pages by every named row and are read once for all of them, through rows[0]; rows that do not share them set
- * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros. Tokens on a page outside the pool are not attended.
+ * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros (one with tokens whose scores are all
+ * -inf NaN, as its softmax is). Tokens on a page outside the pool are not attended.
  * What lies behind a query's tokens has no influence, infinities and NaN included. `out` may be q itself, and lies neither
  * over q in another way nor over the pool.
  * ws: orc_kv_attend_ws bytes of scratch, 16-byte aligned; -1 for a call that no launch can hold (more than 2^24 - 1 workgroups), which orc_kv_attend

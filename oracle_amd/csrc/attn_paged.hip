@@ -59,6 +59,18 @@ __device__ __forceinline__ int visible(const AttendArgs& a, int i, int* row) {
   return ok && lim > 0 ? lim : 0;
 }
 
+// Whether query i has any token to attend, where the sum over its keys came out as 0 (rare: a row without tokens). If it has, all its scores are -inf,
+// and the softmax is 0 / 0.
+__device__ bool attends(const AttendArgs& a, int i) {
+  int r;
+  const int lim = visible(a, i, &r);
+  for (int j = 0; j << a.log_ps < lim; ++j) {
+    const int page = a.table[(size_t)r * a.width + j];
+    if (page >= 0 && page < a.n_pages) return true;
+  }
+  return false;
+}
+
 // the first named row that holds the whole prefix (rows[0] where none does), by one wave
 __device__ __forceinline__ int prefix_row(const AttendArgs& a, int lane) {
   for (int base = 0; base < a.n; base += 64) {
@@ -99,7 +111,7 @@ __device__ __forceinline__ void put(const AttendArgs& a, const Item& it, int col
   if (a.sp + a.ss == 1) {
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
     u32x2 st = {cvt2<T>(v[0] * inv, v[1] * inv), cvt2<T>(v[2] * inv, v[3] * inv)};
-    if (sum == 0.f) st = u32x2{0, 0};
+    if (sum == 0.f) st[0] = st[1] = attends(a, i) ? cvt2<T>(NAN, NAN) : 0;
     *(u32x2*)((T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + d) = st;
   } else {
     const size_t at = ((size_t)i * a.hq + head) * (a.sp + a.ss) + it.part;
@@ -450,6 +462,7 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int i = (int)(id / a.hq), head = (int)(id % a.hq);
   u32x2 st = {cvt2<T>(acc[0] * inv, acc[1] * inv), cvt2<T>(acc[2] * inv, acc[3] * inv)};
+  if (sum == 0.f && attends(a, i)) st[0] = st[1] = cvt2<T>(NAN, NAN);
   *(u32x2*)((T*)a.o + (size_t)i * a.o_ts + (size_t)head * a.o_hs + d) = st;
 }
 

@@ -304,7 +304,7 @@ class KvPages:
         """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
         n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
         once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
-        gives zeros; what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in another way, or over
+        gives zeros (one whose scores are all -inf NaN); what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in another way, or over
         the pool, is refused."""
         _chk(q, 'q', 3, self.dtype, self.device)
         if forward_ad._current_level >= 0:

@@ -111,3 +111,37 @@ def test_reserve_refuses_a_part_page_outside_the_pool(bad):
         assert (slots == -1).all() and all(torch.equal(x, y) for x, y in zip(before, (c.table, c.lens, c.refs)))
     assert (c.reserve(ints([0, 1, 2]), ints([0, 2, 1]), total=3) >= 0).all()      # no token for that row: its page does not matter
     c.check()
+
+
+# Scores of -inf at every token a query sees: the softmax is 0 / 0, as packed_attention has it; a query without tokens keeps its zeros
+@pytest.mark.parametrize('n, prefix, hq, hkv', [(4, 0, 4, 2), (4, 64, 4, 2), (40, 64, 8, 2), (300, 0, 4, 2)])
+def test_scores_of_minus_infinity_alone_give_nan(n, prefix, hq, hkv):
+    hd, own = 64, [(0, 3, 70, 17)[i % 4] for i in range(n)]
+    c, dense = filled(n, prefix, own, 32, hkv, hd, BF, 94)
+    q = torch.randn(n, hq, hd, device=DEV).to(BF)
+    q[..., 5] = q[..., 5].abs() + 1
+    rows, limits = ints(list(range(n))), [prefix + own[i] if i % 3 else (1, 0, prefix + 2)[i // 3 % 3] for i in range(n)]
+    for kh in range(hkv):
+        c2 = KvPages.wrap(c.kv.clone(), c.table, c.lens, c.refs)
+        c2.kv[1, 0, :, kh, :, 5] = float('-inf')
+        for lim in (None, limits):
+            out = c2.attend(1, q, rows, prefix_tokens=prefix, limits=None if lim is None else ints(lim))
+            for i in range(n):
+                m = min(prefix + own[i], prefix + own[i] if lim is None else lim[i])
+                if m <= 0:
+                    assert (out[i] == 0).all()
+                    continue
+                g = slice(kh * hq // hkv, (kh + 1) * hq // hkv)
+                assert out[i, g].isnan().all(), i
+                k, v = (x[:, :m] for x in dense[i])
+                ref, tol = attention64(q[i], k, v, hd ** -0.5)
+                rest = [h for h in range(hq) if not g.start <= h < g.stop]
+                close(out[i, rest], ref[rest], tol[rest], i)
+        c2.check()
+        if not prefix:                                                     # no page of the pool is no token
+            gone = c2.table.clone()
+            gone[2] = -1
+            assert (KvPages.wrap(c2.kv, gone, c.lens, c.refs).attend(1, q, rows)[2] == 0).all()
+    k, v = q[:3, :hkv].clone(), q[:3, :hkv]
+    k[..., 5] = float('-inf')
+    assert packed_attention(q[:3], k, v, PackedPlan([3])).isnan().all()
