@@ -28,6 +28,8 @@ constexpr int KT = 32;            // keys of a wave's tile in keys_item
 constexpr int IDS = 512;          // page ids held in LDS at a time by keys_item
 constexpr int IDS_COLS = 2048;    // by cols_item, whose range has to fit
 constexpr int MAX_SP = 40, MAX_SS = 16;   // parts of a query, of the prefix and of its row's own tokens
+constexpr int UNIT_COLS = 64, UNIT_KEYS = KT;   // keys of a tile: parts of the prefix are whole ones
+static_assert(UNIT_COLS == Tile64<64>::KEYS && UNIT_COLS == Tile64<128>::KEYS);
 static_assert(MAX_SP + MAX_SS <= 64, "a lane of the combining wave each");
 
 struct AttendArgs {
@@ -385,7 +387,7 @@ __global__ __launch_bounds__(256, COLS ? (HD == 64 ? 3 : 2) : 4) void attend_ker
     else { pair = p_at / a.mt; mt = p_at % a.mt; }
     it.kvh = pair % a.hkv;
     it.part = pair / a.hkv;
-    constexpr int UNIT = COLS ? Tile64<HD>::KEYS : KT;
+    constexpr int UNIT = COLS ? UNIT_COLS : UNIT_KEYS;
     const int per = ((a.prefix + UNIT - 1) / UNIT + a.sp - 1) / a.sp * UNIT;
     it.k_lo = it.part * per;
     it.k_hi = it.k_lo + per < a.prefix ? it.k_lo + per : a.prefix;
@@ -494,7 +496,10 @@ Split split_of(const orc_kv_pages* c, int n, int n_heads, int prefix) {
     const int64_t most_sp = (prefix + 255) / 256;
     sp = sp < most_sp ? sp : most_sp;
     sp = sp < 1 ? 1 : sp > MAX_SP ? MAX_SP : sp;
-    s.sp = (int)(s.cols && sp < least_sp ? least_sp : sp);
+    sp = s.cols && sp < least_sp ? least_sp : sp;
+    const int unit = s.cols ? UNIT_COLS : UNIT_KEYS;   // as attend_kernel cuts it; no part is empty (201 tiles in 40 parts are 34 of 6)
+    const int64_t tiles = (prefix + unit - 1) / unit, per = (tiles + sp - 1) / sp;
+    s.sp = (int)((tiles + per - 1) / per);
   }
   const int64_t own = (int64_t)n * c->n_kv_heads * s.gt;
   const int64_t left = (int64_t)c->max_row_pages * c->page_size - prefix;

@@ -109,3 +109,16 @@ def test_attend_refuses_what_no_launch_can_hold(lib, hkv, hq, n, prefix):
     assert lib.orc_kv_attend(C.byref(c), 0, 4096, 4096, st, 4096, None, n, hq, prefix, 0.1, 4096, None) == -1
     assert b'too many' in lib.orc_last_error()
     assert lib.orc_kv_attend_ws(C.byref(c), 1, hkv, 0) >= 0
+
+
+# parts of the prefix whose tiles do not divide by their number: none of them is empty
+@pytest.mark.parametrize('prefix, hkv, hq, n, parts', [
+    (201 * 64, 1, 8, 40, 34 + 13),           # 128 columns at a time, 201 tiles: 34 parts of 6 (not 40, 6 of them empty), and 13 of own tokens
+    (41 * 64, 1, 8, 40, 11 + 13),            # 41: 11 of 4
+    (200 * 64, 2, 8, 40, 40 + 7),            # 40 of 5
+    (16 * 256 + 32, 1, 2, 2, 17 + 16)])      # 16 columns at a time, tiles of 32 keys: 129 in 17 of 8
+def test_no_part_of_a_prefix_is_empty(lib, prefix, hkv, hq, n, parts):
+    fields = dict(kv=1 << 40, table=4096, lens=4096, refs=4096, status=4096, work=4096, n_layers=1, n_pages=4, n_kv_heads=hkv, page_size=32, head_dim=64,
+                  max_rows=4, max_row_pages=4096, dtype=0)
+    c = _lib.OrcKvPages(*[fields[x] for x, _ in _lib.OrcKvPages._fields_])
+    assert lib.orc_kv_attend_ws(C.byref(c), n, hq, prefix) == n * hq * parts * (64 + 2) * 4

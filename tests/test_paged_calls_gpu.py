@@ -145,3 +145,14 @@ def test_scores_of_minus_infinity_alone_give_nan(n, prefix, hq, hkv):
     k, v = q[:3, :hkv].clone(), q[:3, :hkv]
     k[..., 5] = float('-inf')
     assert packed_attention(q[:3], k, v, PackedPlan([3])).isnan().all()
+
+
+@pytest.mark.parametrize('prefix, n, hd', [(201 * 64, 40, 64), (201 * 64, 40, 128), (16 * 256 + 32, 2, 64)])
+def test_attend_prefixes_whose_tiles_do_not_divide_by_their_parts(prefix, n, hd):
+    c, dense = filled(n, prefix, [i % 4 for i in range(n)], 32, 1, hd, BF, 95)
+    q = torch.randn(n, 8 if n > 2 else 2, hd, device=DEV).to(BF)
+    out = c.attend(1, q, ints(list(range(n))), prefix_tokens=prefix)
+    c.check()
+    for i in range(0, n, 7):
+        ref, tol = attention64(q[i], *dense[i], hd ** -0.5)
+        close(out[i], ref, tol, i)
