@@ -23,14 +23,34 @@ _I64x4, _I64x8 = struct.Struct('4q').pack, struct.Struct('8q').pack
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _run(device, name, *args):
-    """The C entry `name` with args and the current stream of `device`, with `device` the current one."""
+class _Held:
+    """Tensors that an object keeps and its calls read on whatever stream is current: noted for every such stream once, so that their memory is not given to
+    others before that stream is through with it when the object is let go. (A captured graph's replays are not noted: who replays it keeps the object.)"""
+
+    def _hold(self, *tensors):
+        self._tensors, self._streams = tensors, set()
+
+    def _note(self, device, stream):
+        if stream in self._streams:
+            return
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                for t in self._tensors:
+                    t.record_stream(torch.cuda.current_stream())
+                self._streams.add(stream)
+
+
+def _run(held, device, name, *args):
+    """The C entry `name` with args and the current stream of `device`, with `device` the current one; it reads the tensors of `held`."""
     fn, i = getattr(_lib.lib(), name), device.index
+    stream = _raw_stream(i)
+    if stream not in held._streams:
+        held._note(device, stream)
     if _current() == i:
-        rc = fn(*args, _raw_stream(i))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(i):
-            rc = fn(*args, _raw_stream(i))
+            rc = fn(*args, stream)
     if rc != 0:
         _lib.check(rc, name)
 
@@ -106,7 +126,7 @@ def _out(out, like, name='out'):
     return out
 
 
-class PackedPlan:
+class PackedPlan(_Held):
     """The query tiles of prompts that lie one behind the other, `lens` tokens each (0 allowed), on `device`: made once for a batch
     and used for every layer. It holds for any number of heads."""
 
@@ -125,6 +145,7 @@ class PackedPlan:
         if lib.orc_attn_plan(arr, n, work.data_ptr(), self.n_work) < 0:
             _lib.check(-1, 'orc_attn_plan')
         self.work = work.to(device)
+        self._hold(self.work)
 
 
 def packed_attention(q, k, v, plan, scale=None, out=None):
@@ -158,12 +179,12 @@ def packed_attention(q, k, v, plan, scale=None, out=None):
     kt, kh, kp = _place(k, 'k')
     vt, vh, vp = _place(v, 'v')
     ot, oh, op = _place(out, 'out')
-    _run(device, 'orc_attention_packed', qp, kp, vp, op, _I64x8(qt, qh, kt, kh, vt, vh, ot, oh), plan.work.data_ptr(), plan.n_work, plan.total,
+    _run(plan, device, 'orc_attention_packed', qp, kp, vp, op, _I64x8(qt, qh, kt, kh, vt, vh, ot, oh), plan.work.data_ptr(), plan.n_work, plan.total,
          hq, hkv, hd, _DTYPES[dtype], scale)
     return out
 
 
-class KvPages:
+class KvPages(_Held):
     """A paged KV cache. kv (n_layers, 2, n_pages, n_kv_heads, page_size, head_dim) holds the tokens; table (max_rows, max_row_pages) the
     pages of every row (-1: none), lens (max_rows,) its tokens, refs (n_pages,) how many rows hold a page -- all on the GPU, so no call waits for it
     and all of them can be captured into a graph. Lists of rows and counts are int32 tensors there. A call whose lists are wrong, or that
@@ -210,6 +231,7 @@ class KvPages:
         self.row_tokens = table.shape[1] * page      # the most a row can hold
         self.status = torch.zeros(1, dtype=torch.int32, device=kv.device)
         self._work = torch.zeros(8 + 4 * n_pages, dtype=torch.int32, device=kv.device)
+        self._hold(kv, table, lens, refs, self.status, self._work)
         self._c = _lib.OrcKvPages(*[t.data_ptr() for t in (kv, table, lens, refs, self.status, self._work)], layers, n_pages, hkv, page, hd,
                                   table.shape[0], table.shape[1], _DTYPES[kv.dtype])
         self._ref = ref = C.byref(self._c)
@@ -223,7 +245,7 @@ class KvPages:
         self._attend_ws = attend_ws
 
     def _call(self, name, *args):
-        _run(self.device, name, self._ref, *args)
+        _run(self, self.device, name, self._ref, *args)
 
     def _rows(self, rows, name='rows', n=None):
         p = _ints(rows, name, self.device, n)
@@ -298,6 +320,8 @@ class KvPages:
         into.check() raises, and nothing is changed."""
         if into is not None and into.device != self.device:
             raise ValueError(f'into is on {into.device}, not on {self.device}')
+        if into is not None:
+            into._note(self.device, _raw_stream(self.device.index))
         self._call('orc_kv_compact', None if into is None else into._ref)
 
     def attend(self, layer, q, rows, prefix_tokens=0, limits=None, scale=None, out=None):

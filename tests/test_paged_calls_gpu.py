@@ -156,3 +156,25 @@ def test_attend_prefixes_whose_tiles_do_not_divide_by_their_parts(prefix, n, hd)
     for i in range(0, n, 7):
         ref, tol = attention64(q[i], *dense[i], hd ** -0.5)
         close(out[i], ref, tol, i)
+
+
+# What a plan or a cache made for itself is not given to others while a stream that used it is still at it
+def test_a_plan_or_cache_let_go_while_another_stream_uses_it():
+    lens = [70, 300]
+    q, k, v = qkv(sum(lens), 4, 2, 64, FP, 96)
+    plan = PackedPlan(lens)
+    want = packed_attention(q, k, v, plan)
+    c, _ = filled(3, 0, [5, 40, 9], 32, 2, 64, FP, 97)
+    rows = ints([0, 1, 2])
+    one, side = c.attend(1, q[:3], rows), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        out, two = packed_attention(q, k, v, plan), c.attend(1, q[:3], rows)
+    held = {t.data_ptr(): t.numel() for t in (plan.work, c.status, c._work)}
+    del plan, c
+    assert not side.query()                                            # still asleep
+    fresh = [torch.empty(n, dtype=torch.int32, device=DEV) for n in held.values() for _ in range(64)]
+    assert not held.keys() & {t.data_ptr() for t in fresh}
+    side.synchronize()
+    assert torch.equal(out, want) and torch.equal(two, one)
