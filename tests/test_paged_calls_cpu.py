@@ -1,5 +1,6 @@
 """CPU: calls of the packed attention and of the paged cache that the C entries have to tell apart before anything is launched."""
 import ctypes as C
+import os
 import random
 
 import pytest
@@ -15,7 +16,8 @@ FAR = (1 << 40, 2 << 40, 3 << 40)
 
 @pytest.fixture(scope='module')
 def lib():
-    __graft_entry__.build()
+    if not os.path.exists(_lib.LIB_PATH):
+        __graft_entry__.build()
     return _lib.lib()
 
 
