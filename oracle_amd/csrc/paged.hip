@@ -142,8 +142,9 @@ __global__ __launch_bounds__(NT) void reserve_kernel(Pages p, const int* rows, c
   }
   int* list = p.work + 8;
   if (!bad) {
-    at = block_scan(pages_of(p, old + add) - pages_of(p, old), &need_all, sh);
-    if (__syncthreads_or(part < 0 || part >= p.n_pages)) bad = ORC_KV_BAD_PAGE;
+    // fewer than 2^20 pages (2^20 tokens in pages of 16, one more a row): what is above counts the bad ones, without a barrier more
+    at = block_scan(pages_of(p, old + add) - pages_of(p, old) + (part < 0 || part >= p.n_pages ? 1 << 20 : 0), &need_all, sh);
+    if (need_all >> 20) bad = ORC_KV_BAD_PAGE;
     else if (need_all > p.n_pages || !lowest_free(p, need_all, list, sh)) bad = ORC_KV_POOL_FULL;
   }
   if (bad) {   // the same for all threads
