@@ -220,13 +220,14 @@ enum { ORC_KV_BAD_ROW = 1, ORC_KV_ROW_TWICE = 2, ORC_KV_BAD_COUNT = 4, ORC_KV_RO
        ORC_KV_BAD_PAGE = 64, ORC_KV_NOT_SHARED = 128 };
 /* counts[i] more tokens (NULL: one) for row rows[i]; slots[0..total): place (page * page_size + offset) of every new token, the rows' tokens
  * one behind the other in list order, -1 behind the last and everywhere when the call fails. A row whose begun page is outside the pool
- * gets no more tokens (ORC_KV_BAD_PAGE). */
+ * gets no more tokens (ORC_KV_BAD_PAGE). The places hold until orc_kv_compact or orc_kv_free of the row. */
 int orc_kv_reserve(const orc_kv_pages* c, const int32_t* rows, const int32_t* counts, int n, int32_t* slots, int total, void* stream);
-/* K / V of `total` tokens (token and head strides in elements) into their slots of one layer; a slot outside the pool is skipped. */
+/* K / V of `total` tokens (token and head strides in elements) into their slots of one layer; a slot outside the pool is skipped. A slot is named once, and
+ * k and v do not lie over the places that are written. */
 int orc_kv_append(const orc_kv_pages* c, int layer, const int32_t* slots, int total, const void* k, const void* v, const int64_t* strides4,
                   void* stream);
 /* Row dst[i] (empty) becomes row src[i], or its first n_tokens tokens (n_tokens < 0: all). share != 0: full pages are shared and the part page
- * is copied; share == 0: every page is copied. A src row may be named more than once. */
+ * is copied; share == 0: every page is copied. A src row may be named more than once. What was reserved for it is appended first, in every layer. */
 int orc_kv_fork(const orc_kv_pages* c, const int32_t* src, const int32_t* dst, int n, int n_tokens, int share, void* stream);
 /* Rows give their pages back (an empty row: nothing). */
 int orc_kv_free(const orc_kv_pages* c, const int32_t* rows, int n, void* stream);
@@ -236,8 +237,8 @@ int orc_kv_free(const orc_kv_pages* c, const int32_t* rows, int n, void* stream)
 int orc_kv_compact(const orc_kv_pages* c, const orc_kv_pages* into, void* stream);
 /* One token of attention per query over the cache: query i (q [n][n_heads][head_dim], strides4 = {q token, q head, out token, out head}) reads
  * the first limits[i] tokens (NULL: all lens[rows[i]]) of row rows[i]. The first prefix_tokens (a multiple of page_size) are held
- * on the same pages by every named row and are read once for all of them, through rows[0]; rows that do not share them set
- * ORC_KV_NOT_SHARED. A query without tokens, or of a row outside the table, gets zeros (one with tokens whose scores are all
+ * on the same pages by every named row and are read once for all of them, through the first named row that holds them all (rows[0] where
+ * none does); rows that do not share them set ORC_KV_NOT_SHARED. A query that ends inside them is right, but makes the call slower (up to three times). A query without tokens, or of a row outside the table, gets zeros (one with tokens whose scores are all
  * -inf NaN, as its softmax is). Tokens on a page outside the pool are not attended.
  * What lies behind a query's tokens has no influence, infinities and NaN included. `out` may be q itself, and lies neither
  * over q in another way nor over the pool.

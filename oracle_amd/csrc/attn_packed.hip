@@ -4,9 +4,11 @@
 // maximum m and sum of one pass over the keys (flash32.h). One workgroup = 4 waves x 32 query rows of one head.
 //
 // Long prompts are bound by the matrix cores and the softmax beside them, at the clock that the power limit leaves (about 1.75 GHz): 2 prompts of 15k
-// and 24k tokens, 32 heads on 8, head dim 128, 5.55 ms = 1183 TFLOP/s, 0.92 of an 8192^3 bf16 product on the same card. Short ones by what a tile costs
-// before its first product (Q, then two K images from HBM) and by the uneven end: 8 prompts of 640..900, 32 heads, 63 us (610 TFLOP/s,
-// 3.2 TB/s); 48 of 0..2304, 16 heads on 4, head dim 64, fp16, 156 us (720 TFLOP/s: half the products to a tile's exponentials).
+// and 24k tokens, 32 heads on 8, head dim 128, 5.8 ms = 1130 TFLOP/s (5.55 to 5.95 ms on different cards), 0.88 of an 8192^3 bf16 product. Short ones by
+// what a tile costs before its first product (Q, then two K images from HBM) and by the uneven end: 8 prompts of 640..900, 32 heads, 68 us (570 TFLOP/s,
+// 3.0 TB/s); 48 of 0..2304, 16 heads on 4, head dim 64, fp16, 164 us (690 TFLOP/s: half the products to a tile's exponentials). Medians of 200 launches one
+// behind the other (40 of the long ones): the first ms of them is faster (157 us a launch of the last case), the next 20 ms up to a third slower, until
+// the clock has settled under the power limit.
 // 128 rows a workgroup and not 256: those halve the reads of K / V, which L2 serves anyway, and leave fewer tiles to spread (measured slower).
 // Two workgroups fit a CU at head dim 128 (256 registers a lane), three at 64 (168).
 #include <algorithm>
@@ -149,7 +151,8 @@ template <typename T, int HD> void launch_hd(const PackedArgs& a, hipStream_t s)
   hipLaunchKernelGGL((packed_kernel<T, HD>), dim3((unsigned)(a.n_work * a.hq)), dim3(256), 0, s, a);
 }
 
-// The tiles of up to kMaxRows prompts, by prompt, written on the device; the prompts longest first, first: tiles before each of them
+// The tiles of up to kMaxRows prompts, by prompt, written on the device; the prompts longest first, first: tiles before each of them. (Without
+// the order by keys that orc_attn_plan gives the last quarter: 3 us of a 7B layer's 1900 at 8 prompts of 640..900.)
 struct PlanArgs { int n, first[kMaxRows + 1], start[kMaxRows], len[kMaxRows]; };
 __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a, int4* work) {
   for (int x = threadIdx.x; x < a.first[a.n]; x += 256) {

@@ -3,18 +3,25 @@
 // out[i] = sum_j p_j v_j / sum_j p_j over the first limits[i] tokens of row rows[i], p_j = exp2(c (q_i . k_j - m)), c = scale * log2(e).
 // The sum is split: the shared prefix is read once for ALL queries of the batch (they are the columns of one matrix product per K/V head),
 // every row's own tokens are read for its n_heads / n_kv_heads query heads. Each part leaves (m, sum, unnormalised output) in fp32;
-// combine_kernel joins the parts of a query by exp2(c (m_part - m)): a launch of its own, 4 us after 18 us of attention for 16 rows over 2304 shared
+// combine_kernel joins the parts of a query by exp2(c (m_part - m)): a launch of its own, 4 us after 19 us of attention for 16 rows over 2304 shared
 // tokens. (The last workgroup of a query could do it; that takes counters cleared before the call and a write-back of every XCD's L2.)
 //
 // Two shapes of work, 4 waves each:
 //   keys_item  16 query columns (one row's heads over its own tokens, or a small batch over the prefix): the waves share the columns and
 //              split the keys. A wave's tile is 32 keys, K straight to registers in operand order, V through 8 KiB of LDS of its own; no
-//              barrier in the loop and little LDS, so 4 workgroups fit a CU and hide each other's memory latency. Bound by HBM: 16 rows of 32 heads, 2304
-//              shared and up to 300 own tokens, 66 MB in 18.5 us = 3.6 TB/s (with hardly a byte to read: 7 us).
+//              barrier in the loop and little LDS, so 4 workgroups fit a CU and hide each other's memory latency. Bound by latency: 16 rows of 32 heads, 2304
+//              shared and up to 300 own tokens, 66 MB in 18.6 us (3.6 TB/s, out of the Infinity Cache where calls follow one another), 7 of
+//              them with hardly a byte to read (launch, lengths, page ids, first tile); over 12 layers in turn, which that cache does not hold, the call
+//              takes 26.7 us instead of 23.0.
 //   cols_item  many columns over the prefix: every wave has 32 columns of its own, 64-key tiles go through a 2-deep LDS ring that
 //              the waves share (flash32.h). Bound by the matrix cores and the softmax between the two products, then by the rows' own tokens: 96 rows of 32
-//              heads on 8, 32k shared and up to 2000 own tokens, 103 us = 510 TFLOP/s and 3.5 TB/s at once (the prefix's items first: own
-//              ones put first or between them were up to twice as slow, the workgroups being dealt out in turn).
+//              heads on 8, 32k shared and up to 2000 own tokens, 108 us = 490 TFLOP/s and 3.3 TB/s at once (the prefix's items first: own
+//              ones put first or between them were up to twice as slow, the workgroups being dealt out in turn). A query that ends inside the prefix
+//              sends every item up to whose end it does not reach to keys_item, 16 columns at a time: that case 127 -> 318 us where one of the
+//              96 ends 100 tokens before the prefix does, 368 where it ends at 16000.
+// The rows' own tokens are cut by the sizes that the host knows (split_of), not by their lengths: MAX_SS parts a row at the most, one from 512 (row, K/V
+// head) pairs on. A batch with one row far longer than the others waits for it: 64 rows of 100 tokens and one of 32k, 8 K/V heads, 427 us (its bytes take
+// 32); one row of 32k alone, 1 / 2 / 8 / 32 K/V heads, 32 / 35 / 37 / 100 us (bytes 3 / 7 / 26 / 105).
 // The page ids of an item's keys are gathered into LDS first, so that the loop's addresses wait for no dependent load.
 #include <type_traits>
 

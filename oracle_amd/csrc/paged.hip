@@ -5,9 +5,10 @@
 // is one workgroup of 1024 threads; what moves tokens is a second launch over all CUs that reads the list of copies the first one left.
 //
 // Such a workgroup is bound by the chain of its loads (lists, lengths, table, counts: about 1 us each, one behind the other) and a dozen barriers, not by
-// bytes: reserve 10.6 us for 8 prompts of 6156 tokens, fork 8.4 us for 24 rows of 2 sources, free 4-5 us, compact's two 4.7 us each. The
-// copies are bound by HBM: append 39 us for a layer of those prompts (200 MB, 5.1 TB/s), compact 354 us (1.77 GB, 5.0 TB/s), whole
-// rows of 16-token pages at head dim 64 111 us (547 MB, 4.9 TB/s).
+// bytes: reserve 9.7 us for 8 prompts of 6156 tokens, fork 8.4 us for 24 rows of 2 sources, free 4-5 us, compact's two 4.8 us each (medians of 200). Of
+// many long rows it is the walk over the table by one CU: fork and free of a row of 2048 pages to 96 rows 320 us. The copies are bound by HBM: append
+// 39 us for a layer of those prompts (200 MB, 5.1 TB/s), compact 357 us (1.77 GB, 5.0 TB/s), whole rows of 16-token pages at head dim 64 113 us (547 MB,
+// 4.8 TB/s).
 #include "../../include/oracle_hip.h"
 #include "kernels.h"
 #include "mma16.h"

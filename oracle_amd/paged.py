@@ -128,7 +128,7 @@ def _out(out, like, name='out'):
 
 class PackedPlan(_Held):
     """The query tiles of prompts that lie one behind the other, `lens` tokens each (0 allowed), on `device`: made once for a batch
-    and used for every layer. It holds for any number of heads."""
+    and used for every layer. It holds for any number of heads. (Making it copies to the GPU and waits: not while a graph is captured.)"""
 
     def __init__(self, lens, device='cuda'):
         self.lens = [int(x) for x in lens]
@@ -263,7 +263,7 @@ class KvPages(_Held):
     def reserve(self, rows, counts=None, total=None):
         """Room for counts[i] more tokens (None: one) of every row: takes the lowest free pages and returns the new tokens' places (int32, `total` of
         them, the rows' tokens one behind the other, -1 behind the last) for `append`. total: the sum of counts, which the host has to know; it
-        may be larger."""
+        may be larger. The places hold until a `compact` in place, or until the row is freed."""
         r = self._rows(rows)
         n = rows.numel()
         c = None if counts is None else _ints(counts, 'counts', self.device, n)
@@ -278,7 +278,8 @@ class KvPages(_Held):
         return slots
 
     def append(self, layer, slots, k, v):
-        """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`, each named once; a place of -1 is skipped."""
+        """k / v (T, n_kv_heads, head_dim) of one layer into the places of `reserve`, each named once; a place of -1 is skipped. k and v may be
+        views of the cache, but not of the places that are written."""
         _chk(k, 'k', 3, self.dtype, self.device)
         _chk(v, 'v', 3, self.dtype, self.device)
         if forward_ad._current_level >= 0:
@@ -303,7 +304,7 @@ class KvPages(_Held):
 
     def fork(self, src, dst, n_tokens=None):
         """The empty rows dst[i] become rows src[i] (their first n_tokens tokens): full pages are shared, the part page is copied. A row can be
-        forked to many; no src row may be among dst."""
+        forked to many; no src row may be among dst. What was reserved for a src row is appended first, in every layer."""
         self._fork(src, dst, n_tokens, 1)
 
     def copy(self, src, dst, n_tokens=None):
@@ -315,9 +316,9 @@ class KvPages(_Held):
         self._call('orc_kv_free', self._rows(rows), rows.numel())
 
     def compact(self, into=None):
-        """Held pages to the front of the pool: in place, the pages that stick out move into the holes. into: another cache of the same geometry
-        (n_pages may differ), which becomes a copy of this one without the holes; this one stays as it is. Too few pages there: a note that
-        into.check() raises, and nothing is changed."""
+        """Held pages to the front of the pool: in place, the pages that stick out move into the holes, and places that `reserve` gave hold no
+        more. into: another cache of the same geometry (n_pages may differ), which becomes a copy of this one without the holes; this one
+        stays as it is. Too few pages there: a note that into.check() raises, and nothing is changed."""
         if into is not None and into.device != self.device:
             raise ValueError(f'into is on {into.device}, not on {self.device}')
         if into is not None:
@@ -327,9 +328,10 @@ class KvPages(_Held):
     def attend(self, layer, q, rows, prefix_tokens=0, limits=None, scale=None, out=None):
         """Attention of one token per query: q (n, Hq, hd), query i over the first limits[i] tokens (None: all) of row rows[i], Hq a multiple of
         n_kv_heads. The first prefix_tokens (a multiple of page_size) are on the same pages in every named row (`fork`) and are read
-        once for all of them. A row can be named more than once (several tokens of a question, with their limits). A query without tokens
-        gives zeros (one whose scores are all -inf NaN); what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in another way, or over
-        the pool, is refused."""
+        once for all of them; a query that ends inside them (by its limit, or a shorter row) makes the call slower, up to three times. A row
+        can be named more than once (several tokens of a question, with their limits). A query without tokens gives zeros (one whose scores are
+        all -inf NaN); what lies behind a query's tokens is not seen, infinities and NaN included. `out` may be q; one that lies over q in
+        another way, or over the pool, is refused."""
         _chk(q, 'q', 3, self.dtype, self.device)
         if forward_ad._current_level >= 0:
             _no_tangents(q=q, out=out)
