@@ -142,7 +142,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void packed_kernel(PackedArg
     __syncthreads();
   }
   T* op = (T*)a.o + (size_t)(seq + qw) * a.o_ts + (size_t)head * a.o_hs;
-  f.template rows<false>(im.of(w), lane, 1.0f / f.total(), [&](int row, int byte, u32x4 v) {
+  const float total = f.total();   // 0: all scores are -inf, the softmax is 0 / 0 (and not 1 / 0, which would pass on an infinity of V)
+  f.template rows<false>(im.of(w), lane, total != 0.f ? 1.f / total : NAN, [&](int row, int byte, u32x4 v) {
     if (qw + row < len) *(u32x4*)((char*)(op + (size_t)row * a.o_ts) + byte) = v;
   });
 }

@@ -17,8 +17,8 @@
 //              the waves share (flash32.h). Bound by the matrix cores and the softmax between the two products, then by the rows' own tokens: 96 rows of 32
 //              heads on 8, 32k shared and up to 2000 own tokens, 108 us = 490 TFLOP/s and 3.3 TB/s at once (the prefix's items first: own
 //              ones put first or between them were up to twice as slow, the workgroups being dealt out in turn). A query that ends inside the prefix
-//              sends every item up to whose end it does not reach to keys_item, 16 columns at a time: that case 127 -> 318 us where one of the
-//              96 ends 100 tokens before the prefix does, 368 where it ends at 16000.
+//              sends every item up to whose end it does not reach to keys_item, 16 columns at a time: 96 rows with own tokens spread evenly
+//              over 0..2000 127 -> 318 us where one of them ends 100 tokens before the prefix does, 368 where it ends at 16000.
 // The rows' own tokens are cut by the sizes that the host knows (split_of), not by their lengths: MAX_SS parts a row at the most, one from 512 (row, K/V
 // head) pairs on. A batch with one row far longer than the others waits for it: 64 rows of 100 tokens and one of 32k, 8 K/V heads, 427 us (its bytes take
 // 32); one row of 32k alone, 1 / 2 / 8 / 32 K/V heads, 32 / 35 / 37 / 100 us (bytes 3 / 7 / 26 / 105).

@@ -178,3 +178,19 @@ def test_a_plan_or_cache_let_go_while_another_stream_uses_it():
     assert not held.keys() & {t.data_ptr() for t in fresh}
     side.synchronize()
     assert torch.equal(out, want) and torch.equal(two, one)
+
+
+# All scores -inf and an infinity in V: 0 / 0 is NaN in every dim, the one of the infinity too
+@pytest.mark.parametrize('hd, dtype', [(128, BF), (64, FP)])
+def test_scores_of_minus_infinity_over_an_infinite_value_give_nan(hd, dtype):
+    for lens in ([1, 1], [3, 70], [64, 130]):
+        q, k, v = (x.clone() for x in qkv(sum(lens), 4, 2, hd, dtype, 98))
+        q[..., 5] = q[..., 5].abs() + 1
+        clean = packed_attention(q, k, v, PackedPlan(lens))
+        k[:lens[0], 1, 5], v[0, 1, 19] = float('-inf'), float('inf')
+        out = packed_attention(q, k, v, PackedPlan(lens))
+        assert out[:lens[0], 2:].isnan().all() and torch.equal(out[:, :2], clean[:, :2]) and torch.equal(out[lens[0]:], clean[lens[0]:])
+        c = KvPages(1, 40, 2, hd, page_size=16, max_rows=2, max_row_pages=20, dtype=dtype)
+        c.append(0, c.reserve(ints([0, 1]), ints(lens), total=sum(lens)), k, v)
+        out = c.attend(0, q[-2:], ints([0, 1]))
+        assert out[0, 2:].isnan().all() and torch.isfinite(out[0, :2]).all() and torch.isfinite(out[1]).all()
