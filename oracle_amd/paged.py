@@ -24,11 +24,12 @@ _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDe
 
 
 class _Held:
-    """Tensors that an object keeps and its calls read on whatever stream is current: noted for every such stream once, so that their memory is not given to
-    others before that stream is through with it when the object is let go. (A captured graph's replays are not noted: who replays it keeps the object.)"""
+    """Tensors that an object keeps and its calls read on whatever stream is current: noted once for every such stream but the one that they were made on, so
+    that their memory is not given to others before that stream is through with it when the object is let go. (A captured graph's replays are not
+    noted: who replays it keeps the object.)"""
 
     def _hold(self, *tensors):
-        self._tensors, self._streams = tensors, set()
+        self._tensors, self._streams = tensors, {_raw_stream(tensors[0].get_device())} if tensors[0].is_cuda else set()
 
     def _note(self, device, stream):
         if stream in self._streams:
